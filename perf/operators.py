@@ -12,7 +12,8 @@ bytes each).  Blocks of 32 along the head dimension have one scale d = m / -8 (m
 largest magnitude, the first of several) and codes min(15, floor(x / d + 8.5)); they stand for
 fp16(d) * (code - 8), d held in 32 bits before it is cut to 16.  Token 8h + g, dimension 32b + 8i + 2c + e of a key is nibble i of halfword e
 of word b in chunk (h, g, c); token 8h + 2c + e, dimension 32b + 8i + g of a value is there too;
-a token's scales are at [h][c][b][e], token 8h + 2c + e."""
+key scales are at [token][b], value
+scales at [h][c][b][e], token 8h + 2c + e."""
 import random
 
 import torch
@@ -131,7 +132,8 @@ def _byte_of(nkv, hd, page, device):
     e = torch.where(kind == 0, w % 2, t % 2)
     code = base + kind * (8 * hd) + ((t // 8 * 8 + g) * 4 + c) * (hd // 8) + b * 4 + e * 2 + i // 2
     blk = torch.arange(hd // 32, device=device).view(1, 1, 1, -1)
-    scale = base + 16 * hd + kind * hd + ((t // 8 * 4 + t % 8 // 2) * (hd // 32) + blk) * 4 + t % 2 * 2
+    paired = ((t // 8 * 4 + t % 8 // 2) * (hd // 32) + blk) * 4 + t % 2 * 2
+    scale = base + 16 * hd + torch.where(kind == 0, (t * (hd // 32) + blk) * 2, hd + paired)
     return code, scale
 
 
@@ -172,7 +174,8 @@ def _values(got, nkv, hd, page):
         y = gr[..., 8 * hd * kind:8 * hd * (kind + 1)].unflatten(-1, (2, 8, 4, nb, 2, 2))
         y = torch.stack((y & 15, y >> 4), -1).flatten(-2).permute(order).reshape(*gr.shape[:3], 16, nb, 32)
         d = gr[..., 16 * hd + hd * kind:16 * hd + hd * (kind + 1)].contiguous().view(torch.float16)
-        d = d.unflatten(-1, (2, 4, nb, 2)).permute(0, 1, 2, 3, 4, 6, 5).reshape(*gr.shape[:3], 16, nb, 1)
+        d = d.unflatten(-1, (2, 4, nb, 2)).permute(0, 1, 2, 3, 4, 6, 5) if kind else d
+        d = d.reshape(*gr.shape[:3], 16, nb, 1)
         out.append(((y.float() - 8.0) * d.float()).flatten(-2).flatten(2, 3).permute(0, 2, 1, 3))
     return out
 
