@@ -540,6 +540,119 @@ int tgx_attn_advance(tgx_attn *a, void *stream);
  * moe (flags TGX_EAGER: launched directly).  TG_EINVAL once the cache is full. */
 int tgx_decode_token(tgx_attn *a, tgx_ctx *moe, float *x_dev, void *stream, int flags);
 
+/* ===================== batched serving: paged 4-bit KV cache, int8 products ===================== */
+
+/* Element types of activations below. */
+#define TGX_F32 0
+#define TGX_BF16 1
+#define TGX_F16 2
+
+/* One layer's keys and values of many sequences, in pages of page_tokens tokens (a
+ * multiple of 16, at most 1024): pages[n_pages] of tgx_kvq_page_bytes bytes each, 16-byte
+ * aligned device memory owned by the caller.  Keys (rotated) and values are held in
+ * blocks of 32 along the head dimension: m = the block's value of the largest magnitude
+ * (the first of several), scale fp16(fp32(m) / -8), codes min(15, floor(8.5 - 8 x / m)),
+ * standing for scale * (code - 8): the Q4_0 rule.  A block with a value that is not finite,
+ * or too large for an fp16 scale, is held as NaN.
+ * A page is [n_kv_heads][page_tokens / 16] granules of 16 tokens, 18 * head_dim bytes each:
+ * key codes | value codes (8 * head_dim bytes each) | key scales | value scales (head_dim
+ * bytes each).  Codes: chunks (h, g, c), h < 2, g < 8, c < 4, of head_dim / 32 32-bit words
+ * b; nibble i of halfword e of a word is, of a key, token 8h + g, dimension
+ * 32b + 8i + 2c + e; of a value, token 8h + 2c + e, dimension 32b + 8i + g.  Scales of
+ * block b: keys [token][b], values [h][c][b][e], token 8h + 2c + e.
+ * head_dim: a multiple of 32, 32 .. 256. */
+typedef struct {
+    void *pages;
+    int n_pages;
+    int page_tokens;
+    int n_kv_heads;
+    int head_dim;
+} tgx_kvq_cache;
+
+/* The sequences of one call, on the device (graphs replay with new contents):
+ * q_start[n_seqs + 1]: sequence b has the new tokens q_start[b] .. q_start[b + 1] - 1 of the
+ * call's token rows (none is allowed; rows behind q_start[n_seqs] are left as they are);
+ * kv_lens[n_seqs]: its cached rows, the new ones included, so new token i of n is row
+ * kv_lens - n + i; page_table[n_seqs][max_pages]: the page of rows page_tokens * j ..., read
+ * up to the sequence's last row only.  max_new: no sequence has more new tokens (> 0; 1 for
+ * a decode step).  status: a device word or NULL, 0 at first; calls or in TGX_KVQ_BAD_* when
+ * the contents do not fit: a page id outside the cache or a length beyond the table (such
+ * rows are neither written nor attended to), a new token with a negative row or a rope
+ * position outside the tables (not written, its outputs 0), more new tokens than max_new
+ * (not attended: left as they are). */
+typedef struct {
+    int n_seqs;
+    int max_pages;
+    int max_new;
+    const int32_t *q_start;
+    const int32_t *kv_lens;
+    const int32_t *page_table;
+    int32_t *status;
+} tgx_kvq_batch;
+#define TGX_KVQ_BAD_PAGE 1
+#define TGX_KVQ_BAD_LENGTH 2
+#define TGX_KVQ_BAD_POSITION 4
+#define TGX_KVQ_BAD_NEW 8
+
+/* Bytes of one page, or 0 for a shape the cache does not take. */
+size_t tgx_kvq_page_bytes(int n_kv_heads, int head_dim, int page_tokens);
+
+/* The new tokens' heads, per token t: q_out[t] = rope(norm(q[t])), and rope(norm(k[t])) and
+ * v[t] into the cache at the token's row (the batched form of the norm, RoPE and append
+ * steps of tg_attention_decode, csrc/libtinygiant.c:380-400).  q [n_tokens][n_heads *
+ * head_dim], k and v [n_tokens][n_kv_heads * head_dim] of `dtype`, rows *_stride elements
+ * apart; q_out dense.  q_norm / k_norm: fp32 [head_dim] RMSNorm weights, or NULL for no
+ * norm; rope_cos / rope_sin: fp32 [n_pos][head_dim / 2], or NULL for no rotation; the
+ * position is the token's row, or positions[t] when given (device int32).  n_heads = 0 and
+ * q = NULL: keys and values only.  q_out may be q (dense); it must not overlap k or v.
+ * Two new tokens must not fall on the same page row.  All rows 4-element aligned (4 *
+ * element size), strides multiples of 4.  Keys are computed in 64 bits, so codes are the
+ * definition's; q in 32. */
+int tgx_kvq_append(const tgx_kvq_cache *cache, const tgx_kvq_batch *batch, int dtype, int n_tokens, const void *q,
+                   long long q_stride, const void *k, long long k_stride, const void *v, long long v_stride,
+                   int n_heads, const float *q_norm, const float *k_norm, float eps, const float *rope_cos,
+                   const float *rope_sin, int n_pos, const int32_t *positions, void *q_out, void *stream);
+
+/* The values the cache holds for the batch's new tokens: k_out / v_out [n_tokens][n_kv_heads]
+ * [head_dim] fp32 (either may be NULL); 0 for a row that is not in the cache.  A batch whose
+ * new tokens are a sequence's whole length reads all of it. */
+int tgx_kvq_read(const tgx_kvq_cache *cache, const tgx_kvq_batch *batch, int n_tokens, float *k_out, float *v_out,
+                 void *stream);
+
+/* out[t][h] = sum_r softmax_r(scale * q[t][h] . k_r) v_r over the rows r <= the token's own
+ * row, kv head h / (n_heads / n_kv_heads) (tg_attention_decode's scores, softmax and V sum,
+ * csrc/libtinygiant.c:402-445, for many tokens over the 4-bit cache).  q and out
+ * [n_tokens][n_heads * head_dim] of `dtype`, rows *_stride elements apart (4-element aligned;
+ * strides multiples of 4); out may be q.  scale: 0 selects 1 / sqrt(head_dim).  A token without a row
+ * to attend to (kv_lens 0) gets 0.  n_heads / n_kv_heads <= 32.  Sums and softmax statistics
+ * are fp32.  scratch: tgx_kvq_attention_scratch_bytes bytes, 256-byte aligned, no contents
+ * assumed or kept; calls sharing it must be ordered. */
+size_t tgx_kvq_attention_scratch_bytes(const tgx_kvq_cache *cache, const tgx_kvq_batch *batch, int n_tokens,
+                                       int n_heads);
+int tgx_kvq_attention(const tgx_kvq_cache *cache, const tgx_kvq_batch *batch, int dtype, int n_tokens, const void *q,
+                      long long q_stride, int n_heads, void *out, long long out_stride, float scale, void *scratch,
+                      size_t scratch_bytes, void *stream);
+
+/* 8-bit integer rows: codes int8 [rows][tgx_i8_row_bytes(cols)] (zeros behind cols), one
+ * fp32 scale per row.  y = x (norm_w NULL) or x * norm_w; codes rint(127 y / max |y|) (ties
+ * to even), scale max |y| / 127, with norm_w times the RMSNorm factor 1 / sqrt(mean x^2 +
+ * eps): codes * scale stands for the row, or for its RMSNorm.  A row with a value that is not
+ * finite gets scale NaN and codes 0; a zero row scale 0.  x: rows x_stride elements apart.
+ * codes 16-byte aligned. */
+size_t tgx_i8_row_bytes(int cols);
+int tgx_i8_quantize_rows(int dtype, const void *x, long long x_stride, int rows, int cols, const float *norm_w,
+                         float eps, int8_t *codes, float *scales, void *stream);
+
+/* out[m][n] = sum_k a[m][k] w[n][k] * (sa[m] * sw[n]) (+ residual[m][n]): a, sa the rows of x
+ * quantised as above (norm_w NULL or the RMSNorm in front), w, sw int8 rows and scales of
+ * tgx_i8_quantize_rows (16-byte aligned).  The integer sum is exact (k <= 131072); the rest
+ * fp32, rounded once to `dtype`.  residual may be out.  scratch: tgx_i8_matmul_scratch_bytes
+ * bytes, 256-byte aligned, no contents assumed or kept; calls sharing it must be ordered. */
+size_t tgx_i8_matmul_scratch_bytes(int m, int n, int k);
+int tgx_i8_matmul(int dtype, const void *x, long long x_stride, int m, int k, const float *norm_w, float eps,
+                  const int8_t *w_codes, const float *w_scales, int n, const void *residual, long long res_stride,
+                  void *out, long long out_stride, void *scratch, size_t scratch_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

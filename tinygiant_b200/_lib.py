@@ -40,6 +40,15 @@ TGX_KQ_CHAINED = 1
 TGX_EAGER = 1
 TGX_MULTI = 2
 
+TGX_F32 = 0
+TGX_BF16 = 1
+TGX_F16 = 2
+
+TGX_KVQ_BAD_PAGE = 1
+TGX_KVQ_BAD_LENGTH = 2
+TGX_KVQ_BAD_POSITION = 4
+TGX_KVQ_BAD_NEW = 8
+
 LIB_NAME = "libtinygiant.so"
 
 
@@ -52,6 +61,15 @@ class TinyGiantError(RuntimeError):
 class TgxShape(ctypes.Structure):
     _fields_ = [("embed", CI), ("inter", CI), ("n_experts", CI), ("top_k", CI), ("n_layers", CI),
                 ("rms_eps", CF)]
+
+
+class TgxKvqCache(ctypes.Structure):
+    _fields_ = [("pages", VP), ("n_pages", CI), ("page_tokens", CI), ("n_kv_heads", CI), ("head_dim", CI)]
+
+
+class TgxKvqBatch(ctypes.Structure):
+    _fields_ = [("n_seqs", CI), ("max_pages", CI), ("max_new", CI), ("q_start", VP), ("kv_lens", VP),
+                ("page_table", VP), ("status", VP)]
 
 
 # name -> (restype, argtypes); the order follows include/tinygiant.h
@@ -164,6 +182,15 @@ PROTOTYPES = {
     "tgx_fused_debug": (CI, [VP, VP, VP, SZ]),
     "tgx_fused_trace": (CI, [VP, VP, VP, VP]),
     "tgx_last_routing": (CI, [VP, CI, VP, VP, VP]),
+    "tgx_kvq_page_bytes": (SZ, [CI, CI, CI]),
+    "tgx_kvq_append": (CI, [VP, VP, CI, CI, VP, LL, VP, LL, VP, LL, CI, VP, VP, CF, VP, VP, CI, VP, VP, VP]),
+    "tgx_kvq_read": (CI, [VP, VP, CI, VP, VP, VP]),
+    "tgx_kvq_attention_scratch_bytes": (SZ, [VP, VP, CI, CI]),
+    "tgx_kvq_attention": (CI, [VP, VP, CI, CI, VP, LL, CI, VP, LL, CF, VP, SZ, VP]),
+    "tgx_i8_row_bytes": (SZ, [CI]),
+    "tgx_i8_quantize_rows": (CI, [CI, VP, LL, CI, CI, VP, CF, VP, VP, VP]),
+    "tgx_i8_matmul_scratch_bytes": (SZ, [CI, CI, CI]),
+    "tgx_i8_matmul": (CI, [CI, VP, LL, CI, CI, VP, CF, VP, VP, CI, VP, LL, VP, LL, VP, SZ, VP]),
 }
 
 
