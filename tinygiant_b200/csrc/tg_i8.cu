@@ -8,6 +8,10 @@
 // |y| and the sum of squares.  A code is cut at borders k + 1/2: it is first taken in fp32
 // and, where that lands near a border, decided again in 64 bits, so codes are the
 // definition's.
+#include <cuda.h>
+
+#include <cmath>
+
 #include "tg_serve.cuh"
 
 namespace tg {
@@ -42,6 +46,7 @@ __global__ void __launch_bounds__(QT) k_i8_rows(QuantArgs a) {
     __shared__ double s_top[QT / 32];
     __shared__ float s_ss[QT / 32];
     __shared__ int s_bad;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the product's weights may come
     const int row = blockIdx.x, tid = threadIdx.x;
     const T* x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.xs;
     double top = 0.0;
@@ -98,41 +103,399 @@ __global__ void __launch_bounds__(QT) k_i8_rows(QuantArgs a) {
     }
 }
 
+// ---------------------------------------------------------------- the product
+//
+// tcgen05.mma kind::i8, int32 accumulators in TMEM.  The weights' rows (output channels) are
+// the MMA's 128 rows and the tokens its columns, so a lane of the epilogue is a channel:
+// outputs of 32 neighbouring channels leave together for any stride, sw[n] is one register,
+// and few tokens cost few columns.  Operands come by TMA, K in steps of 128 bytes, 128-byte
+// swizzle, into a ring of stages; rows and bytes beyond the matrices are filled with zeros.
+//
+// Warps 0 .. 3 are the epilogue (TMEM lanes 32 w ..), warp 4 issues the copies, warp 5 the
+// MMAs.  A CTA walks its tiles; with two accumulators the epilogue of one runs behind the
+// MMAs of the next.  Where there are fewer tiles than SMs, K is split over the CTAs of a
+// cluster: each puts its int32 sums into its own shared memory, and every CTA adds up and
+// finishes every splits-th column, exactly, whatever the split.
+//
+// The first copies of weights are issued before the quantiser in front has finished.
+// Every wait is bounded; where one expires the tile's outputs become NaN, copies and MMAs in
+// flight are waited for (bounded) and the TMEM is freed.
 struct MatArgs {
-    const int8_t* a;
     const float* sa;
-    const int8_t* w;
     const float* sw;
-    int M, N, kp;
+    int M, N;
     const void* res;
     long long rs;
     void* out;
     long long os;
+    int tn;       // tokens per tile, a multiple of 16 up to 256
+    int ksteps;   // 128-byte steps of a row
+    int stages;
+    int splits;   // CTAs of a cluster that share a tile
 };
 
-template <int DT>
-__global__ void __launch_bounds__(256) k_i8_dot(MatArgs g) {
-    using T = typename Elem<DT>::T;
-    const int lane = threadIdx.x & 31, n = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (n >= g.N) return;
-    for (int m = blockIdx.y; m < g.M; m += gridDim.y) {
-        const int4* a = reinterpret_cast<const int4*>(g.a + (size_t)m * g.kp);
-        const int4* w = reinterpret_cast<const int4*>(g.w + (size_t)n * g.kp);
-        int acc = 0;
-        for (int i = lane; i < g.kp / 16; i += 32) {
-            const int4 u = a[i], v = w[i];
-            acc = __dp4a(u.x, v.x, acc);
-            acc = __dp4a(u.y, v.y, acc);
-            acc = __dp4a(u.z, v.z, acc);
-            acc = __dp4a(u.w, v.w, acc);
-        }
-        acc = __reduce_add_sync(0xffffffffu, acc);
-        if (lane == 0) {
-            float o = (float)acc * (g.sa[m] * g.sw[n]);
-            if (g.res) o += to_f32(reinterpret_cast<const T*>(g.res)[(size_t)m * g.rs + n]);
-            from_f32(o, reinterpret_cast<T*>(g.out)[(size_t)m * g.os + n]);
+constexpr int TM = 128;           // channels per tile
+constexpr int KB = 128;           // bytes of K per stage
+constexpr int MAX_STAGES = 12;
+constexpr int GT = 192;           // threads
+constexpr long long WAIT_CYCLES = 2000000000ll;   // about a second
+
+__device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(uint64_t* m, int n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(saddr(m)), "r"(n));
+}
+__device__ __forceinline__ void mbar_expect(uint64_t* m, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(saddr(m)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* m) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(saddr(m)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t* m, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(saddr(m)), "r"(parity)
+        : "memory");
+    return done;
+}
+// Waits for the phase; false once the limit is over here or a wait has failed elsewhere in the CTA.
+__device__ __forceinline__ bool mbar_wait(uint64_t* m, uint32_t parity, volatile int* failed) {
+    if (mbar_try(m, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try(m, parity)) {
+        if (*failed) return false;
+        if (clock64() - t0 > WAIT_CYCLES) {
+            *failed = 1;
+            return false;
         }
     }
+    return true;
+}
+// The same for what must land before the CTA may end.
+__device__ __forceinline__ void mbar_drain(uint64_t* m, uint32_t parity) {
+    const long long t0 = clock64();
+    while (!mbar_try(m, parity) && clock64() - t0 < WAIT_CYCLES) {
+    }
+}
+
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, uint64_t* mbar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            saddr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(saddr(mbar))
+        : "memory");
+}
+
+// K-major operand in 128-byte swizzle: rows of 128 bytes, 8-row atoms 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t (&v)[N], uint32_t at);
+template <>
+__device__ __forceinline__ void tmem_ld<16>(uint32_t (&v)[16], uint32_t at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(at));
+}
+
+template <int DT>
+__global__ void __launch_bounds__(GT, 1)
+    k_i8_mma(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mx, MatArgs g) {
+    using T = typename Elem<DT>::T;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_free[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_failed;
+    uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    volatile int* failed = &s_failed;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int nt = (g.N + TM - 1) / TM, mt = (g.M + g.tn - 1) / g.tn, tiles = nt * mt;
+    const int rank = (int)blockIdx.x % g.splits, first = (int)blockIdx.x / g.splits, stride = (int)gridDim.x / g.splits;
+    const int k0 = (int)((long long)g.ksteps * rank / g.splits), k1 = (int)((long long)g.ksteps * (rank + 1) / g.splits);
+    const int stage_bytes = TM * KB + g.tn * KB;
+    uint32_t cols = 32;
+    while ((int)cols < 2 * g.tn) cols *= 2;
+
+    if (tid == 0) {
+        for (int i = 0; i < g.stages; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_free[i], 128);
+        }
+        s_failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;");
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&s_tmem)), "r"(cols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+
+    if (warp == 4) {
+        if (lane == 0) {
+            // x is the quantiser's: only weights may be fetched before it has finished
+            const int n_mine = first < tiles ? (tiles - first + stride - 1) / stride : 0;
+            const int ahead = min(g.stages, n_mine * (k1 - k0));
+            for (int f = 0; f < ahead; f++) {
+                const int tile = first + f / (k1 - k0) * stride, k = k0 + f % (k1 - k0);
+                mbar_expect(&full[f], stage_bytes);
+                tma_load(sm + f * stage_bytes, &mw, k * KB, tile % nt * TM, &full[f]);
+            }
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            int f = 0, issued = 0;
+            bool ok = true;
+            for (int tile = first; tile < tiles && ok; tile += stride)
+                for (int k = k0; k < k1 && ok; k++, f++) {
+                    const int s = f % g.stages;
+                    uint8_t* at = sm + s * stage_bytes;
+                    if (f >= ahead) {
+                        ok = mbar_wait(&empty[s], (f / g.stages - 1) & 1, failed);
+                        if (!ok) break;
+                        mbar_expect(&full[s], stage_bytes);
+                        tma_load(at, &mw, k * KB, tile % nt * TM, &full[s]);
+                    }
+                    tma_load(at + TM * KB, &mx, k * KB, tile / nt * g.tn, &full[s]);
+                    issued = f + 1;
+                }
+            if (*failed || !ok)   // everything that is under way lands before the CTA ends
+                for (int i = max(0, issued - g.stages); i < issued; i++) mbar_drain(&full[i % g.stages], (i / g.stages) & 1);
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            // D int32, A and B signed, K-major, N = tn, M = 128
+            const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(g.tn >> 3) << 17) | ((TM >> 4) << 24);
+            int f = 0, i = 0;
+            bool ok = true;
+            for (int tile = first; tile < tiles && ok; tile += stride, i++) {
+                if (i >= 2) ok = mbar_wait(&acc_free[i & 1], ((i >> 1) - 1) & 1, failed);
+                const uint32_t d = tmem + (i & 1) * (cols / 2);
+                for (int k = k0; k < k1 && ok; k++, f++) {
+                    const int s = f % g.stages;
+                    ok = mbar_wait(&full[s], (f / g.stages) & 1, failed);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t da = sw128_desc(saddr(sm + s * stage_bytes));
+                    const uint64_t db = sw128_desc(saddr(sm + s * stage_bytes + TM * KB));
+#pragma unroll
+                    for (int x = 0; x < KB / 32; x++)
+                        asm volatile(
+                            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                            "l"(da + 2 * x), "l"(db + 2 * x), "r"(idesc), "r"((k > k0 || x) ? 1 : 0));
+                    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                                     saddr(&empty[s]))
+                                 : "memory");
+                }
+                if (ok)
+                    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                                     saddr(&acc_full[i & 1]))
+                                 : "memory");
+            }
+            if (!ok)   // the last stages' MMAs
+                for (int x = max(0, f - g.stages); x < f; x++) mbar_drain(&empty[x % g.stages], (x / g.stages) & 1);
+        }
+    } else {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        T* out = reinterpret_cast<T*>(g.out);
+        const T* res = reinterpret_cast<const T*>(g.res);
+        int i = 0;
+        for (int tile = first; tile < tiles; tile += stride, i++) {
+            const int m0 = tile / nt * g.tn, n = tile % nt * TM + 32 * warp + lane;
+            const bool n_ok = n < g.N;
+            const float sw = n_ok ? g.sw[n] : 0.0f;
+            const bool ok = mbar_wait(&acc_full[i & 1], (i >> 1) & 1, failed);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t d = tmem + (i & 1) * (cols / 2) + ((uint32_t)(32 * warp) << 16);
+            if (g.splits > 1) {
+                // own sums to shared memory (its stages are no longer in use), [column][channel]
+                int* part = reinterpret_cast<int*>(sm);
+                for (int c = 0; c < g.tn && ok; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld<16>(v, d + c);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int x = 0; x < 16; x++) part[(c + x) * TM + 32 * warp + lane] = (int)v[x];
+                }
+                break;   // one tile per cluster
+            }
+            for (int c = 0; c < g.tn && m0 + c < g.M; c += 16) {
+                uint32_t v[16];
+                tmem_ld<16>(v, d + c);
+                const int m = m0 + c + (lane & 15);
+                const float sal = m < g.M ? g.sa[m] : 0.0f;
+                float r[16];
+                if (res)
+#pragma unroll
+                    for (int x = 0; x < 16; x++)
+                        r[x] = n_ok && m0 + c + x < g.M ? to_f32(res[(size_t)(m0 + c + x) * g.rs + n]) : 0.0f;
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int x = 0; x < 16; x++) {
+                    const float sa = __shfl_sync(0xffffffffu, sal, x);
+                    float o = (float)(int)v[x] * (sa * sw);
+                    if (res) o += r[x];
+                    if (!ok) o = __int_as_float(0x7fc00000);
+                    if (n_ok && m0 + c + x < g.M) from_f32(o, out[(size_t)(m0 + c + x) * g.os + n]);
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            mbar_arrive(&acc_free[i & 1]);
+        }
+    }
+    __syncwarp();
+    if (g.splits > 1) {   // every CTA's sums are in shared memory
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (warp < 4 && first < tiles) {
+            T* out = reinterpret_cast<T*>(g.out);
+            const T* res = reinterpret_cast<const T*>(g.res);
+            const int m0 = first / nt * g.tn, n = first % nt * TM + 32 * warp + lane;
+            const float sw = n < g.N ? g.sw[n] : 0.0f;
+            bool bad = false;
+            for (int r = 0; r < g.splits; r++) {
+                uint32_t at, v;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(saddr(&s_failed)), "r"(r));
+                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+                bad |= v != 0;
+            }
+            for (int c = rank; c < g.tn && m0 + c < g.M; c += g.splits) {
+                int acc = 0;
+                const uint32_t mine = saddr(sm) + (uint32_t)(c * TM + 32 * warp + lane) * 4;
+                for (int r = 0; r < g.splits; r++) {
+                    uint32_t at, v;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine), "r"(r));
+                    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+                    acc += (int)v;
+                }
+                if (n < g.N) {
+                    float o = (float)acc * (g.sa[m0 + c] * sw);
+                    if (res) o += to_f32(res[(size_t)(m0 + c) * g.rs + n]);
+                    if (bad) o = __int_as_float(0x7fc00000);
+                    from_f32(o, out[(size_t)(m0 + c) * g.os + n]);
+                }
+            }
+        }
+        // nobody leaves while its sums may still be read
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
+}
+
+// ---------------------------------------------------------------- its launch
+constexpr int SMEM_MAX = 227 * 1024 - 2048;   // beside the barriers
+
+struct MatPlan {
+    int tn, splits, stages, ctas;
+};
+
+// The tile's tokens and the split of K, by an estimate in SM cycles: a K step of 128 bytes
+// takes the MMAs' 2 per token (128 at least: the weights' tile is read through shared memory)
+// or its bytes' way at about 32 bytes a cycle and SM, whichever is longer; a tile's last
+// columns leave at about 8 a token, and a split adds its exchange.
+MatPlan plan_mat(int M, int N, int kp, int sms) {
+    const int nt = (N + TM - 1) / TM, kt = (kp + KB - 1) / KB;
+    MatPlan best{};
+    double best_cost = 1e300;
+    for (int tn = 16; tn <= 256; tn += 16) {
+        if (tn > 16 && tn - 16 >= M) break;   // wider than the tokens
+        const long long tiles = (long long)nt * ((M + tn - 1) / tn);
+        const double step = fmax(fmax(2.0 * tn, 128.0), (TM * KB + tn * KB) / 32.0);
+        for (int s = 1; s <= 8 && s <= kt; s++) {
+            if (s > 1 && (tiles * s > sms || tn * TM * 4 > SMEM_MAX - 1024)) break;
+            const long long waves = (tiles * s + sms - 1) / sms;
+            const double cost = (double)waves * ((kt + s - 1) / s) * step + 8.0 * tn + (s > 1 ? 1500.0 + 4.0 * tn : 0.0);
+            if (cost < best_cost) {
+                best_cost = cost;
+                const long long ctas = tiles * s < sms ? tiles * s : sms;
+                best = MatPlan{tn, s, 0, (int)ctas};
+            }
+        }
+    }
+    const int stage = TM * KB + best.tn * KB;
+    best.stages = (SMEM_MAX - 1024) / stage;
+    if (best.stages > MAX_STAGES) best.stages = MAX_STAGES;
+    return best;
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return (EncodeTiled)p;
+    }();
+    return fn;
+}
+
+// int8 rows of kp bytes, copied in boxes of 128 bytes by `box` rows.
+bool row_map(CUtensorMap* m, const void* base, int rows, int kp, int box) {
+    const cuuint64_t dims[2] = {(cuuint64_t)kp, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)kp};
+    const cuuint32_t boxes[2] = {KB, (cuuint32_t)box}, ones[2] = {1, 1};
+    return encode_tiled()(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, boxes, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 0;
+    return sms;
+}
+
+template <int DT>
+cudaError_t launch_mat(MatArgs g, const int8_t* x, const int8_t* w, int kp, cudaStream_t s) {
+    const int sms = sm_count();
+    if (!sms || !encode_tiled()) return cudaErrorNotSupported;
+    const MatPlan p = plan_mat(g.M, g.N, kp, sms);
+    g.tn = p.tn;
+    g.splits = p.splits;
+    g.stages = p.stages;
+    g.ksteps = (kp + KB - 1) / KB;
+    CUtensorMap mw, mx;
+    if (!row_map(&mw, w, g.N, kp, TM) || !row_map(&mx, x, g.M, kp, p.tn)) return cudaErrorInvalidValue;
+    const int ring = p.stages * (TM * KB + p.tn * KB), part = p.splits > 1 ? p.tn * TM * 4 : 0;
+    const int smem = (ring > part ? ring : part) + 1024;
+    cudaError_t e = cudaFuncSetAttribute(k_i8_mma<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.ctas);
+    cfg.blockDim = dim3(GT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.splits;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, k_i8_mma<DT>, mw, mx, g);
 }
 
 template <int DT>
@@ -202,14 +565,9 @@ extern "C" int tgx_i8_matmul(int dtype, const void* x, long long x_stride, int m
     tg::QuantArgs qa{x, x_stride, m, k, kp, norm_w, eps, codes, scales};
     cudaError_t e = tg::launch_rows(dtype, qa, s);
     if (e != cudaSuccess) return tg::serve_fail(TG_ECUDA, fn, cudaGetErrorString(e));
-    tg::MatArgs g{codes, scales, w_codes, w_scales, m, n, kp, residual, res_stride, out, out_stride};
-    const dim3 grid((n + 7) / 8, m < 4096 ? m : 4096);
-    if (dtype == TGX_F32)
-        tg::k_i8_dot<TGX_F32><<<grid, 256, 0, s>>>(g);
-    else if (dtype == TGX_BF16)
-        tg::k_i8_dot<TGX_BF16><<<grid, 256, 0, s>>>(g);
-    else
-        tg::k_i8_dot<TGX_F16><<<grid, 256, 0, s>>>(g);
-    SERVE_LAUNCHED(fn);
-    return TG_OK;
+    tg::MatArgs g{scales, w_scales, m, n, residual, res_stride, out, out_stride, 0, 0, 0, 0};
+    e = dtype == TGX_F32    ? tg::launch_mat<TGX_F32>(g, codes, w_codes, kp, s)
+        : dtype == TGX_BF16 ? tg::launch_mat<TGX_BF16>(g, codes, w_codes, kp, s)
+                            : tg::launch_mat<TGX_F16>(g, codes, w_codes, kp, s);
+    return e == cudaSuccess ? TG_OK : tg::serve_fail(TG_ECUDA, fn, cudaGetErrorString(e));
 }
