@@ -97,14 +97,14 @@ def norm_rope(x, w, eps, cos, sin):
 
 def attention(q, k, v, scale):
     """q [n][NH][hd], k / v [L][NKV][hd] float64; query i sees rows 0 .. L - n + i.  Returns the
-    output, sum p |v|, the largest sum |q||k| scale, per (query, head), and sum p max |v| over each
-    block's values."""
+    output, sum p |v|, the largest sum |q||k| scale and the largest |v|, per (query, head)."""
     n, nh, hd = q.shape
     L, nkv = k.shape[:2]
-    out, spread, reach = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(q)
+    out, spread = torch.zeros_like(q), torch.zeros_like(q)
     size = torch.zeros(n, nh, 1, dtype=q.dtype, device=q.device)
+    top = torch.zeros_like(size)
     if not L:
-        return out, spread, size, reach
+        return out, spread, size, top
     seen = torch.arange(L, device=q.device)[None] <= (L - n + torch.arange(n, device=q.device))[:, None]
     for h in range(nh):
         j = h // (nh // nkv)
@@ -112,9 +112,9 @@ def attention(q, k, v, scale):
         ok = seen.any(1)
         p = torch.softmax(s[ok], 1)
         out[ok, h], spread[ok, h] = p @ v[:, j], p @ v[:, j].abs()
-        reach[ok, h] = p @ v[:, j].abs().unflatten(-1, (-1, 32)).amax(-1).repeat_interleave(32, -1)
+        top[ok, h] = v[:, j].abs().max()
         size[ok, h] = ((q[ok, h].abs() @ k[:, j].abs().T) * scale).masked_fill(~seen[ok], 0).amax(1, keepdim=True)
-    return out, spread, size, reach
+    return out, spread, size, top
 
 
 def i8_rows(x, norm=None, eps=0.0):

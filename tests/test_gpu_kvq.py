@@ -64,20 +64,21 @@ class Setup:
         return [torch.cat(x) for x in zip(*parts)]
 
 
-def close(got, ref, spread, size, reach, hd, rows, dtype):
+def close(got, ref, spread, size, top, hd, rows, dtype):
     """fp32 path: a score sums hd products (each rounding 2^-24 of sum |q||k| = size) and is
     subtracted and scaled in fp32 (4 more of |s| <= size); p carries twice that and exp's 2 units;
     the sum over the rows and its norm `rows` roundings of sum p|v| each.  16-bit types: q, k, v
-    and p may be held in 11 bits (2^-11 each at most) in front of the fp32 sums, and a value's code
-    and its offset of 8 may be summed apart: sum c p d - 8 sum p d, each mma of 16 rows adding 17
-    numbers cut at 2^-24 of an exponent field up to 2^10 above p d, so both together are off by
-    2 * 17 * 2^-14 sum p d < 2^-11 sum p (8 d), 8 d being the block's largest value (reach).  Then
-    one rounding to the type."""
+    and p may be held in 11 bits (2^-11 each at most) in front of the fp32 sums.  A probability is
+    held in fp16 pieces, 2^6 at the largest one, whose last bit is 2^-24: each is off by up to
+    2^-25 / 2^6 of the largest besides, whatever its own size, so an output by rows * 2^-31 * the
+    largest |v| (seen where a peaked row's value is 0 and what is left is smaller still).  Then one
+    rounding to the type."""
     u = 2.0 ** -24
     ds = (hd + 8) * u * size
     tol = spread * (2 * ds + (2 * rows + 32) * u)
     if dtype != F32:
-        tol = tol + spread * (4 * 2.0 ** -11 * size + 3 * 2.0 ** -11) + 2.0 ** -11 * reach
+        tol = tol + spread * (4 * 2.0 ** -11 * size + 3 * 2.0 ** -11)
+    tol = tol + rows * 2.0 ** -31 * top
     tol = tol + 1.001 * R.EPS[dtype] * (ref.abs() + tol) + 1e-30
     d = (got.double() - ref).abs()
     assert torch.isfinite(got.float()).all()

@@ -13,16 +13,17 @@
 // fp32 inputs keep 22 bits of q and of p * d as two fp16 pieces, each an mma of its own; for
 // 16-bit types one piece (11 bits) is as fine as the output.  The pieces stay in fp16's range
 // by powers of two: q's rows are scaled to 2^13 .. 2^14, p to 2^6 at its maximum, V scales to
-// 2^2 .. 2^5 at the largest met so far (vexp; O is rescaled when a larger one comes).
+// 2^2 .. 2^5 at the largest met so far (vexp; O is rescaled when a larger one comes).  So a
+// probability below 2^-31 of its row's largest counts as 0.
 //
-// Codes become fp16 by masks.  For 16-bit types a nibble masked into the low byte of a
-// halfword IS the number code * 2^-24 (a subnormal; 2^-20 for the nibble above it): eight
-// codes cost four ANDs and a shift.  The upper nibbles' factor 16 is taken off q, and off the
-// output; the codes' offset of 8 is -8 sum q in the scores' first accumulator and, for V, one
-// more mma per block whose other operand is -8 * 2^-24 throughout.  The tensor cores align
-// products by exponent fields, which subnormals leave 2^6 .. 2^10 above their values, so sums
-// are good to about 2^-17: below 16-bit outputs, too coarse for fp32.  There the nibbles go
-// into the low bits of 1024 and one half-precision operation more makes them code - 8.
+// Codes become fp16 by masks: a nibble in the low bits of 1024, and one half-precision
+// operation makes it code - 8.  K's codes with 16-bit types go without the second: a nibble
+// masked into the low byte of a halfword IS the number code * 2^-24 (a subnormal; 2^-20 for
+// the nibble above it).  The upper nibbles' factor 16 is taken off q, and the codes' offset is
+// -8 sum q, the scores' first accumulator.  (The tensor cores align products by exponent
+// fields, which subnormals leave 2^6 .. 2^10 above their values, so such a sum is good to about
+// 2^-17 of sum |q| 16 d: enough for a score behind 16-bit inputs, too coarse for fp32, and for
+// V, where sum 8 p d would have to cancel.)
 //
 // Work: an item is (sequence, kv head, tile of 8 * NT query rows), its units the granules
 // of 16 tokens (18 * HD contiguous bytes).  All items' units in one line are cut into equal
@@ -58,30 +59,43 @@ struct AttnKvqArgs {
     void* out;
     long long os;
     float scale;        // times log2(e)
+    uint32_t k1024;     // fp16 1024 twice
     int workers;
     float* slots;       // [workers][2] partial results: m, l [rows], O [rows][HD]
     int* heads;         // [workers][2][4] what a slot holds: kind, token row base, kv head, query rows
 };
 
 // Slot kinds: nothing; a part that its item goes on behind; the item's last part.
+constexpr int MAX_SMS = 160;
+constexpr int workers_per_sm(int warps) { return warps > 1 ? 4 : 12; }
+constexpr int MAX_WORKERS = MAX_SMS * workers_per_sm(1);
+
 enum { SLOT_NONE = 0, SLOT_MORE = 1, SLOT_LAST = 2 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d = a b + c
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                         const float (&e)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(e[0]), "f"(e[1]), "f"(e[2]), "f"(e[3]));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // an 8 x 8 tile of halves across the warp
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
-    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
@@ -89,16 +103,56 @@ __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast
 
 // Two codes of the lower (bits 0 .. 3 of each halfword) or the upper nibbles (4 .. 7) as
 // fp16: code - 8, or, RAW, code * 2^-24 and code * 2^-20.
+// `k1024` is 1024 twice, in a register: one three-input operation then masks and merges.
 template <bool RAW>
-__device__ __forceinline__ uint32_t codes_lo(uint32_t x) {
+__device__ __forceinline__ uint32_t codes_lo(uint32_t x, uint32_t k1024) {
     if constexpr (RAW) return x & 0x000f000fu;
-    return as_u32(__hadd2(as_h2((x & 0x000f000fu) | 0x64006400u), __float2half2_rn(-1032.0f)));
+    uint32_t y;
+    asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(y) : "r"(x), "r"(k1024));
+    return as_u32(__hadd2(as_h2(y), __float2half2_rn(-1032.0f)));
 }
 template <bool RAW>
-__device__ __forceinline__ uint32_t codes_hi(uint32_t x) {
+__device__ __forceinline__ uint32_t codes_hi(uint32_t x, uint32_t k1024) {
     if constexpr (RAW) return x & 0x00f000f0u;
-    return as_u32(__hfma2(as_h2((x & 0x00f000f0u) | 0x64006400u), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f)));
+    uint32_t y;
+    asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xEA;" : "=r"(y) : "r"(x), "r"(k1024));
+    return as_u32(__hfma2(as_h2(y), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f)));
 }
+
+constexpr uint32_t NO_GRANULE = 0xffffffffu;
+
+// N words, in the widest loads that their alignment allows.
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<uint4*>(&w[i]) = *reinterpret_cast<const uint4*>(p + 4 * i);
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) *reinterpret_cast<uint2*>(&w[i]) = *reinterpret_cast<const uint2*>(p + 4 * i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
+    }
+}
+// N fp16 scales as floats.
+template <int N>
+__device__ __forceinline__ void load_scales(float (&d)[N], const uint8_t* p) {
+    if constexpr (N % 2 == 0) {
+        uint32_t w[N / 2];
+        load_words<N / 2>(w, p);
+#pragma unroll
+        for (int i = 0; i < N; i++) d[i] = i & 1 ? __high2float(as_h2(w[i / 2])) : __low2float(as_h2(w[i / 2]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) d[i] = __half2float(*reinterpret_cast<const __half*>(p + 2 * i));
+    }
+}
+__device__ __forceinline__ float2 load2(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 load2(const __nv_bfloat16* p) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
+}
+__device__ __forceinline__ float2 load2(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
 
 // A sequence's share of the call.
 struct SeqInfo {
@@ -107,6 +161,11 @@ struct SeqInfo {
     int off;            // new token i sees the rows below off + i + 1 (may be negative)
     int tiles, grans;   // row tiles per kv head; units per tile (at least one)
 };
+
+__device__ __forceinline__ long long quotient(long long x, long long y) {
+    if ((x | y) < 0x100000000ll) return (uint32_t)x / (uint32_t)y;
+    return x / y;
+}
 
 __device__ __forceinline__ SeqInfo seq_info(const AttnKvqArgs& a, int b, int tile_rows) {
     SeqInfo s;
@@ -123,22 +182,25 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnKvqArgs& a, int b, int til
     return s;
 }
 
-template <int NB> constexpr int stages() { return NB <= 4 ? 4 : 3; }
+// Four CTAs of four warps per SM (128 registers a thread) where that leaves nothing to spill.
+constexpr int min_ctas(int nb, int nt) { return nb <= 3 && nt == 1 ? 4 : nb * nt <= 4 ? 3 : 2; }
+
+constexpr int STAGES = 3;
+constexpr int U = 2;   // granules of a stage, and of a step of the loop
 
 // Shared memory of a CTA of W warps: the rings, which the joining of the warps reuses.
 template <int NB, int NT>
 constexpr int attn_smem(int W) {
-    const int ring = W * stages<NB>() * 18 * 32 * NB, join = W * 8 * NT * (32 * NB + 4) * 4;
+    const int ring = W * STAGES * U * 18 * 32 * NB, join = W * 8 * NT * (32 * NB + 4) * 4;
     return ring > join ? ring : join;
 }
 
 template <int DT, int NB, int NT>
-__global__ void __launch_bounds__(32 * DEEP_WARPS) k_kvq_attn(AttnKvqArgs a) {
+__global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(AttnKvqArgs a) {
     using T = typename Elem<DT>::T;
-    constexpr int HD = 32 * NB, GB = 18 * HD, ST = stages<NB>(), KS = 2 * NB, ROWS = 8 * NT;
+    constexpr int HD = 32 * NB, GB = 18 * HD, ST = STAGES, KS = 2 * NB, ROWS = 8 * NT;
     constexpr int PC = DT == TGX_F32 ? 2 : 1;    // fp16 pieces of q and of p * d
-    constexpr bool RAW = PC == 1;                // codes as subnormals
-    constexpr int OC = RAW ? NB : 1;             // offset accumulators
+    constexpr bool RAW = PC == 1;                // K's codes as subnormals
     extern __shared__ __align__(16) uint8_t sm[];
     __shared__ long long s_scan[8];
     __shared__ long long s_base;
@@ -175,11 +237,12 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS) k_kvq_attn(AttnKvqArgs a) {
         if (i < wid) before += s_scan[i];
         total += s_scan[i];
     }
-    // at least one granule per warp of a worker: short work goes to fewer workers
-    const long long used = max(1ll, min((long long)a.workers, (total + W - 1) / W));
+    // at least one step per warp of a worker: short work goes to fewer workers
+    const long long used = max(1ll, min((long long)a.workers, quotient(total + U * W - 1, U * W)));
     const long long w = blockIdx.x;
-    long long u = w < used ? total * w / used : total;
-    const long long u_end = w < used ? total * (w + 1) / used : total;
+    const long long share = quotient(total, used), more = total - share * used;   // `more` workers have one unit more
+    long long u = w < used ? share * w + min(w, more) : total;
+    const long long u_end = w < used ? u + share + (w < more ? 1 : 0) : total;
     if (tid < 2) {   // no slots yet
         a.heads[((size_t)w * 2 + tid) * 4] = SLOT_NONE;
     }
@@ -200,7 +263,8 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS) k_kvq_attn(AttnKvqArgs a) {
     int b = s_seq;
     long long base = s_base;   // units in front of sequence b
 
-    uint8_t* ring = sm + wid * ST * GB;
+    uint8_t* ring = sm + wid * ST * U * GB;
+    const uint32_t k1024 = a.k1024;
     while (u < u_end) {
         const SeqInfo si = seq_info(a, b, ROWS);
         const long long units = (long long)si.tiles * si.grans * a.c.nkv;
@@ -209,17 +273,71 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS) k_kvq_attn(AttnKvqArgs a) {
             b++;
             continue;
         }
-        const int item = (int)((u - base) / si.grans), g0 = (int)((u - base) % si.grans);
+        const int item = (int)quotient(u - base, si.grans), g0 = (int)(u - base - (long long)item * si.grans);
         const int rt = item / a.c.nkv, j = item % a.c.nkv;   // kv heads innermost
         const int g1 = (int)min((long long)si.grans, g0 + (u_end - u));
         u += g1 - g0;
         const int row0 = rt * ROWS, nrows = min(ROWS, si.n * a.R - row0);   // query rows of the item
 
+        // rows that new token i attends to: those below its limit
+        auto limit = [&](int i) { return (int)max(0ll, min(si.len, (long long)si.off + i + 1)); };
+        const int lim_min = limit(row0 / a.R), lim_max = limit((row0 + nrows - 1) / a.R);
+
+        // ---- this warp's granules below the last visible row: U from g0 + U wid on, U from
+        // g0 + U (wid + W) on, ..., in nk steps
+        const int gl = min(g1, (lim_max + 15) >> 4);
+        const int nk = gl > g0 + U * wid ? (gl - g0 - U * wid + U * W - 1) / (U * W) : 0;
+        const int gpp = a.c.pt >> 4;
+        // lane l: the 32 x + l'th of them, counted through all pages, or NO_GRANULE
+        auto find = [&](int x) -> uint32_t {
+            const int k = 32 * x + lane, gi = g0 + U * (wid + k / U * W) + k % U;
+            if (gi >= gl) return NO_GRANULE;
+            const int pi = gi / gpp;
+            const int page = a.b.table[(size_t)b * a.b.max_pages + pi];
+            if (page < 0 || page >= a.c.n_pages) {
+                kvq_flag(a.b, TGX_KVQ_BAD_PAGE);
+                return NO_GRANULE;
+            }
+            return ((uint32_t)page * a.c.nkv + j) * gpp + (gi - pi * gpp);
+        };
+        // two sets of 32; the one behind is refilled when the front has moved on
+        uint32_t at_even = find(0), at_odd = find(1);
+        uint32_t there = 0;   // U bits per step: the granules that exist, the step issued last lowest
+        // one commit group per call; a granule that does not exist becomes zeros
+        auto issue = [&](int k) {
+            const uint8_t* src[U];
+            uint32_t size[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint32_t at = __shfl_sync(0xffffffffu, k * U & 32 ? at_odd : at_even, (k * U + u) & 31);
+                const bool ok = at != NO_GRANULE;   // none behind the last step either
+                there = there << 1 | (ok ? 1u : 0u);
+                size[u] = ok ? 16 : 0;
+                src[u] = a.c.pages + (size_t)(ok ? at : 0) * GB;
+            }
+            const uint32_t dst = smem_addr(ring + (k % ST) * (U * GB)) + 16 * lane;
+            constexpr int C = GB / 16;   // pieces of a granule
+#pragma unroll
+            for (int i = 0; i < (U * C + 31) / 32; i++) {
+                const int o = 32 * i + lane;
+                const int first = 32 * i / C, last = min(U * C - 1, 32 * i + 31) / C;   // granules of this round
+                const int u = first == last ? first : o >= last * C ? last : first;
+                const uint8_t* from = (first == last ? src[first] : o >= last * C ? src[last] : src[first]) + 16 * (o - u * C);
+                const uint32_t n = first == last ? size[first] : o >= last * C ? size[last] : size[first];
+                if (32 * i + 32 <= U * C || o < U * C)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 512 * i), "l"(from), "r"(n)
+                                 : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int k = 0; k < ST - 1; k++) issue(k);
+
         // ---- the query rows as B operands: lane (g, c) holds row g's dimensions 16s + 2c, + 1
         // and + 8, and the rows' factors, limits and offsets for the columns 2c, 2c + 1
         uint32_t qf[NT][PC][KS][2];
-        float corr[NT][NB][2], fac[NT][2];
-        int lim[NT][2], lim_min = 0x7fffffff, lim_max = 0;
+        float corr[NT][NB][4], fac[NT][2];
+        int lim[NT][2], lim_g[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const int r = 8 * n + g;
@@ -231,9 +349,11 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS) k_kvq_attn(AttnKvqArgs a) {
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    x[s][h] = ok ? to_f32(src[16 * s + 8 * (h >> 1) + 2 * c + (h & 1)]) : 0.0f;
-                    top = fmaxf(top, fabsf(x[s][h]));
+                for (int h = 0; h < 2; h++) {
+                    const float2 y = ok ? load2(src + 16 * s + 8 * h + 2 * c) : make_float2(0.0f, 0.0f);
+                    x[s][2 * h] = y.x;
+                    x[s][2 * h + 1] = y.y;
+                    top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
                 }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -259,15 +379,13 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS) k_kvq_attn(AttnKvqArgs a) {
                 }
             float f = a.scale * (RAW ? 0x1p24f : 1.0f);
             f = scalbnf(f, e);
-            int l = (int)max(0ll, min(si.len, (long long)si.off + (ok ? rho / a.R : 0) + 1));
-            if (!ok) l = 0x7fffffff;   // rows beyond the item: any scores will do
+            const int l = ok ? limit(rho / a.R) : 0x7fffffff;   // rows beyond the item: any scores will do
+            lim_g[n] = l;
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 fac[n][k] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + k));
                 lim[n][k] = __shfl_sync(0xffffffffu, l, 4 * (2 * c + k));
             }
-            lim_min = min(lim_min, l);
-            lim_max = max(lim_max, ok ? l : 0);
 #pragma unroll
             for (int i = 0; i < NB; i++) {
                 float t = sums[i];
@@ -275,211 +393,168 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS) k_kvq_attn(AttnKvqArgs a) {
                 t += __shfl_xor_sync(0xffffffffu, t, 2);
                 t = RAW ? t * (-8.0f * 0x1p-24f) : 0.0f;
 #pragma unroll
-                for (int k = 0; k < 2; k++) corr[n][i][k] = __shfl_sync(0xffffffffu, t, 4 * (2 * c + k));
-            }
-        }
-#pragma unroll
-        for (int o = 16; o >= 4; o >>= 1) {
-            lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
-            lim_max = max(lim_max, __shfl_xor_sync(0xffffffffu, lim_max, o));
-        }
-
-        // ---- this warp's granules: g0 + wid, + W, ... below the last visible row
-        const int gl = min(g1, (lim_max + 15) >> 4);
-        const int nk = gl > g0 + wid ? (gl - g0 - wid + W - 1) / W : 0;
-        const int gpp = a.c.pt >> 4;
-        // lane l: where granule 32 x + l of this warp lies, or -1
-        auto find = [&](int x) -> long long {
-            const int k = 32 * x + lane;
-            if (k >= nk) return -1;
-            const int gi = g0 + wid + k * W, pi = gi / gpp;
-            const int page = a.b.table[(size_t)b * a.b.max_pages + pi];
-            if (page < 0 || page >= a.c.n_pages) {
-                kvq_flag(a.b, TGX_KVQ_BAD_PAGE);
-                return -1;
-            }
-            return (long long)((size_t)page * a.c.page_bytes + (size_t)(j * gpp + gi - pi * gpp) * GB);
-        };
-        long long at_cur = find(0), at_next = find(1);
-        auto issue = [&](int k) {   // one commit group per call
-            const long long at = __shfl_sync(0xffffffffu, (k >> 5) & 1 ? at_next : at_cur, k & 31);
-            if (k < nk && at >= 0) {
-                const uint8_t* src = a.c.pages + at;
-                const uint32_t dst = smem_addr(ring + (k % ST) * GB);
-#pragma unroll
-                for (int i = 0; i < (GB / 16 + 31) / 32; i++) {
-                    const int o = 32 * i + lane;
-                    if (o < GB / 16)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 16 * o), "l"(src + 16 * o)
-                                     : "memory");
+                for (int k = 0; k < 2; k++) {
+                    corr[n][i][k] = __shfl_sync(0xffffffffu, t, 4 * (2 * c + k));
+                    // a register of its own: the accumulator's four are read together
+                    asm volatile("mov.f32 %0, %1;" : "=f"(corr[n][i][k + 2]) : "f"(corr[n][i][k]));
                 }
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
+        }
 
-        float m[NT][2], l[NT][2], o[NT][2 * NB][4], oc[NT][OC][4];
+        float m[NT][2], off[NT][2], l[NT][2], o[NT][2 * NB][4];   // off = P_EXP - m
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
-            for (int k = 0; k < 2; k++) m[n][k] = -INFINITY, l[n][k] = 0.0f;
+            for (int k = 0; k < 2; k++) m[n][k] = -INFINITY, off[n][k] = INFINITY, l[n][k] = 0.0f;
 #pragma unroll
             for (int t = 0; t < 2 * NB; t++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) o[n][t][k] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < OC; t++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) oc[n][t][k] = 0.0f;
         }
-        int vexp = -100;                         // V scales are held times 2^-vexp
-        __half2 vmul = __float2half2_rn(0.0f);   // that factor (two of them: 2^-vexp may leave fp16)
-        __half2 vmul2 = vmul;
+        int vexp = 0;                            // V scales are held times 2^-vexp
+        __half2 vmul = __float2half2_rn(1.0f);   // that factor
+        uint32_t vlim = 0;                       // fp16 bits of 2^(V_HIGH + vexp), the largest scale that fits; none yet
 
-#pragma unroll
-        for (int k = 0; k < ST - 1; k++) issue(k);
+#pragma unroll 1
         for (int k = 0; k < nk; k++) {
             asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
             __syncwarp();
-            const long long at = __shfl_sync(0xffffffffu, (k >> 5) & 1 ? at_next : at_cur, k & 31);
-            // the lanes' places: two sets of 32, the one behind refilled when the front moves on
-            if ((k & 31) == 0 && k) {
-                if ((k >> 5) & 1) at_cur = find((k >> 5) + 1);
-                else at_next = find((k >> 5) + 1);
+            if (k && (k * U & 31) == 0) {
+                if (k * U & 32) at_even = find(k * U / 32 + 1);
+                else at_odd = find(k * U / 32 + 1);
             }
             issue(k + ST - 1);
-            if (at < 0) continue;
-            const uint8_t* gr = ring + (k % ST) * GB;
-            const int t0 = (g0 + wid + k * W) * 16;
+            const uint32_t have = there >> ((ST - 1) * U);   // bit U - 1 - u: granule u of this step
+            const uint8_t* step = ring + (k % ST) * (U * GB);
+            const int t0 = (g0 + U * (wid + k * W)) * 16;
 
             // ---- scores
-            float sc[NT][4];
+            float sc[U][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int u = 0; u < U; u++) {
+                const uint8_t* gr = step + u * GB;
+                uint32_t kw[2][NB];
+                float kd[2][NB];
 #pragma unroll
-                for (int x = 0; x < 4; x++) sc[n][x] = 0.0f;
-            const uint32_t* kc = reinterpret_cast<const uint32_t*>(gr) + lane * NB;   // chunk (h, g, c): word h * 32 * NB
-            const __half* ks = reinterpret_cast<const __half*>(gr + 16 * HD) + g * NB;
-            uint32_t kw[2][NB];
-            float kd[2][NB];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if constexpr (NB % 4 == 0) {
-#pragma unroll
-                    for (int i = 0; i < NB; i += 4)
-                        *reinterpret_cast<uint4*>(&kw[h][i]) = *reinterpret_cast<const uint4*>(kc + h * 32 * NB + i);
-                } else if constexpr (NB % 2 == 0) {
-#pragma unroll
-                    for (int i = 0; i < NB; i += 2)
-                        *reinterpret_cast<uint2*>(&kw[h][i]) = *reinterpret_cast<const uint2*>(kc + h * 32 * NB + i);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NB; i++) kw[h][i] = kc[h * 32 * NB + i];
+                for (int h = 0; h < 2; h++) {
+                    load_words<NB>(kw[h], gr + (h * 32 + lane) * NB * 4);
+                    load_scales<NB>(kd[h], gr + 16 * HD + (h * 8 + g) * NB * 2);
                 }
-                if constexpr (NB % 2 == 0) {
 #pragma unroll
-                    for (int i = 0; i < NB; i += 2) {
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(ks + h * 8 * NB + i));
-                        kd[h][i] = f.x;
-                        kd[h][i + 1] = f.y;
+                for (int i = 0; i < NB; i++) {
+                    const uint32_t w0 = kw[0][i], w1 = kw[1][i], x0 = w0 >> 8, x1 = w1 >> 8;
+                    const uint32_t a0[4] = {codes_lo<RAW>(w0, k1024), codes_lo<RAW>(w1, k1024), codes_hi<RAW>(w0, k1024),
+                                            codes_hi<RAW>(w1, k1024)};
+                    const uint32_t a1[4] = {codes_lo<RAW>(x0, k1024), codes_lo<RAW>(x1, k1024), codes_hi<RAW>(x0, k1024),
+                                            codes_hi<RAW>(x1, k1024)};
+                    constexpr float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        float acc[4];
+                        if constexpr (RAW)
+                            mma16816(acc, a0, qf[n][0][2 * i][0], qf[n][0][2 * i][1], corr[n][i]);
+                        else
+                            mma16816(acc, a0, qf[n][0][2 * i][0], qf[n][0][2 * i][1], none);
+                        mma16816(acc, a1, qf[n][0][2 * i + 1][0], qf[n][0][2 * i + 1][1]);
+#pragma unroll
+                        for (int p = 1; p < PC; p++) {
+                            mma16816(acc, a0, qf[n][p][2 * i][0], qf[n][p][2 * i][1]);
+                            mma16816(acc, a1, qf[n][p][2 * i + 1][0], qf[n][p][2 * i + 1][1]);
+                        }
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+                            sc[u][n][x] = i ? fmaf(kd[x >> 1][i], acc[x], sc[u][n][x]) : kd[x >> 1][i] * acc[x];
                     }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NB; i++) kd[h][i] = __half2float(ks[h * 8 * NB + i]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < NB; i++) {
-                const uint32_t w0 = kw[0][i], w1 = kw[1][i], x0 = w0 >> 8, x1 = w1 >> 8;
-                const uint32_t a0[4] = {codes_lo<RAW>(w0), codes_lo<RAW>(w1), codes_hi<RAW>(w0), codes_hi<RAW>(w1)};
-                const uint32_t a1[4] = {codes_lo<RAW>(x0), codes_lo<RAW>(x1), codes_hi<RAW>(x0), codes_hi<RAW>(x1)};
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    float acc[4] = {corr[n][i][0], corr[n][i][1], corr[n][i][0], corr[n][i][1]};
-#pragma unroll
-                    for (int p = 0; p < PC; p++) {
-                        mma16816(acc, a0, qf[n][p][2 * i][0], qf[n][p][2 * i][1]);
-                        mma16816(acc, a1, qf[n][p][2 * i + 1][0], qf[n][p][2 * i + 1][1]);
-                    }
-                    sc[n][0] = fmaf(kd[0][i], acc[0], sc[n][0]);
-                    sc[n][1] = fmaf(kd[0][i], acc[1], sc[n][1]);
-                    sc[n][2] = fmaf(kd[1][i], acc[2], sc[n][2]);
-                    sc[n][3] = fmaf(kd[1][i], acc[3], sc[n][3]);
                 }
             }
 
-            // ---- p = 2^(s - m + P_EXP); m moves when a score is beyond its slack
-            bool over = false;
+            // ---- t = s - m + P_EXP; is one beyond the slack in m's range?
+            float t[U][NT][4];
+            constexpr uint32_t ALL = (1u << U) - 1;
+            const bool edge = t0 + 16 * U > lim_min || (have & ALL) != ALL;
+            auto sees = [&](int u, int n, int x) {   // whether the column's row attends to the lane's token
+                return t0 + 16 * u + g + 8 * (x >> 1) < lim[n][x & 1] && (have >> (U - 1 - u) & 1);
+            };
+            auto place = [&] {
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+                for (int u = 0; u < U; u++)
 #pragma unroll
-                for (int x = 0; x < 4; x++) sc[n][x] *= fac[n][x & 1];
-            if (t0 + 16 > lim_min) {
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int x = 0; x < 4; x++) t[u][n][x] = fmaf(sc[u][n][x], fac[n][x & 1], off[n][x & 1]);
+                if (edge) {
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int x = 0; x < 4; x++)
+                                if (!sees(u, n, x)) t[u][n][x] = -INFINITY;
+                }
+            };
+            place();
+            float top_t = t[0][0][0];
+#pragma unroll
+            for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int x = 0; x < 4; x++)
-                        if (t0 + g + 8 * (x >> 1) >= lim[n][x & 1]) sc[n][x] = -INFINITY;
-            }
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int x = 0; x < 4; x++) over |= sc[n][x] > m[n][x & 1] + P_SLACK;
+                    for (int x = 0; x < 4; x++) top_t = fmaxf(top_t, t[u][n][x]);
+            bool odd = top_t > P_EXP + P_SLACK;
 
-            // ---- V scales: pairs of tokens, the lane's own; larger ones than fit, or not finite?
-            const uint32_t* vs = reinterpret_cast<const uint32_t*>(gr + 17 * HD) + c * NB;
-            uint32_t vd[2][NB];
-            __half2 vtop = __float2half2_rn(0.0f);
+            // ---- V scales: does one not fit, or is not finite?  A word of two for each lane.
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if constexpr (NB % 4 == 0) {
+            for (int u = 0; u < U; u++)
 #pragma unroll
-                    for (int i = 0; i < NB; i += 4)
-                        *reinterpret_cast<uint4*>(&vd[h][i]) = *reinterpret_cast<const uint4*>(vs + h * 4 * NB + i);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NB; i++) vd[h][i] = vs[h * 4 * NB + i];
+                for (int i = 0; i < (NB + 3) / 4; i++) {
+                    const int x = 32 * i + lane;
+                    if (NB % 4 == 0 || x < 8 * NB) {
+                        const uint32_t v = *reinterpret_cast<const uint32_t*>(step + u * GB + 17 * HD + 4 * x) & 0x7fff7fffu;
+                        odd |= max(v & 0xffffu, v >> 16) > vlim;
+                    }
                 }
-#pragma unroll
-                for (int i = 0; i < NB; i++) vtop = __hmax2_nan(vtop, __habs2(as_h2(vd[h][i])));
-            }
-            const float vt = fmaxf(__low2float(vtop), __high2float(vtop));
-            const bool vnan = !(__low2float(vtop) <= 65504.0f) || !(__high2float(vtop) <= 65504.0f);
-            // rows behind the limits hold anything: their NaN must not reach a product
-            const bool odd = __any_sync(0xffffffffu, over || vnan || vt > scalbnf(1.0f, V_HIGH + vexp));
             bool mend = false;
-            if (odd) {
-                mend = __any_sync(0xffffffffu, vnan);
-                float top = vnan ? 0.0f : vt;
-                if (mend) {   // the largest finite one
+            if (__any_sync(0xffffffffu, odd)) {
+                bool nan = false;
+                float top = 0.0f;   // the largest finite one
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                for (int u = 0; u < U; u++)
 #pragma unroll
-                        for (int i = 0; i < NB; i++) {
-                            const float x = fabsf(__low2float(as_h2(vd[h][i]))), y = fabsf(__high2float(as_h2(vd[h][i])));
-                            if (x <= 65504.0f) top = fmaxf(top, x);
-                            if (y <= 65504.0f) top = fmaxf(top, y);
+                    for (int i = 0; i < (NB + 3) / 4; i++) {
+                        const int x = 32 * i + lane;
+                        if (x < 8 * NB) {
+                            const __half2 v = __habs2(*reinterpret_cast<const __half2*>(step + u * GB + 17 * HD + 4 * x));
+                            const float v0 = __low2float(v), v1 = __high2float(v);
+                            nan |= !(v0 <= 65504.0f) || !(v1 <= 65504.0f);
+                            top = fmaxf(top, fmaxf(v0 <= 65504.0f ? v0 : 0.0f, v1 <= 65504.0f ? v1 : 0.0f));
                         }
-                }
+                    }
+                mend = __any_sync(0xffffffffu, nan);
 #pragma unroll
                 for (int x = 16; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                 float vf = 1.0f;
-                if (top > scalbnf(1.0f, V_HIGH + vexp)) {
-                    const int e = max(ilogbf(top) - V_LOW, -30);
-                    vf = scalbnf(1.0f, max(vexp - e, -126));
+                if (top > __half2float(__ushort_as_half((uint16_t)vlim))) {
+                    const int e = min(max(ilogbf(top) - V_LOW, -14), 13);
+                    vf = scalbnf(1.0f, vexp - e);
                     vexp = e;
-                    vmul = __float2half2_rn(scalbnf(1.0f, -(vexp / 2)));
-                    vmul2 = __float2half2_rn(scalbnf(1.0f, -(vexp - vexp / 2)));
+                    vmul = __float2half2_rn(scalbnf(1.0f, -e));
+                    vlim = V_HIGH + e >= 16 ? 0x7bffu : (uint32_t)__half_as_ushort(__float2half_rn(scalbnf(1.0f, V_HIGH + e)));
                 }
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
                     for (int k2 = 0; k2 < 2; k2++) {
-                        float t = fmaxf(sc[n][k2], sc[n][k2 + 2]);
+                        float mn = m[n][k2];
 #pragma unroll
-                        for (int x = 16; x >= 4; x >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
-                        const float mn = fmaxf(m[n][k2], t);
+                        for (int u = 0; u < U; u++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++)
+                                if (sees(u, n, k2 + 2 * h)) mn = fmaxf(mn, sc[u][n][k2 + 2 * h] * fac[n][k2]);
+#pragma unroll
+                        for (int x = 16; x >= 4; x >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
                         const float f = mn == m[n][k2] ? 1.0f : ex2(m[n][k2] - mn);
                         m[n][k2] = mn;
+                        off[n][k2] = P_EXP - mn;
                         l[n][k2] *= f;
                         const float of = f * vf;
 #pragma unroll
@@ -487,93 +562,82 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS) k_kvq_attn(AttnKvqArgs a) {
                             o[n][t2][k2] *= of;
                             o[n][t2][k2 + 2] *= of;
                         }
-#pragma unroll
-                        for (int t2 = 0; t2 < OC; t2++) {
-                            oc[n][t2][k2] *= of;
-                            oc[n][t2][k2 + 2] *= of;
-                        }
                     }
                 }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int i = 0; i < NB; i++) vd[h][i] = as_u32(__hmul2(__hmul2(as_h2(vd[h][i]), vmul), vmul2));
-
-            // ---- p in pieces, transposed: lane (g, c) gets row g's tokens 2c, 2c + 1 of each half
-            uint32_t ph[NT][PC][2];
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                float p[4];
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    // nothing seen yet leaves m at -inf: masked scores are 0, NaN stays NaN
-                    p[x] = sc[n][x] == -INFINITY ? 0.0f : ex2(sc[n][x] - (m[n][x & 1] - P_EXP));
-                    l[n][x & 1] += p[x];
-                    // beside a NaN a probability that fp16 would lose stays above zero
-                    if (mend && sc[n][x] > -INFINITY) p[x] = fmaxf(p[x], 0x1p-24f);
-                }
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const __half2 hi = __floats2half2_rn(p[2 * h], p[2 * h + 1]);
-                    ph[n][0][h] = transpose8(as_u32(hi));
-                    if constexpr (PC == 2)
-                        ph[n][1][h] = transpose8(
-                            as_u32(__floats2half2_rn(p[2 * h] - __low2float(hi), p[2 * h + 1] - __high2float(hi))));
-                }
+                place();
             }
 
-            // ---- O += (p d) V
-            const uint32_t* vc = reinterpret_cast<const uint32_t*>(gr + 8 * HD) + lane * NB;
-            uint32_t vw[2][NB];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if constexpr (NB % 4 == 0) {
-#pragma unroll
-                    for (int i = 0; i < NB; i += 4)
-                        *reinterpret_cast<uint4*>(&vw[h][i]) = *reinterpret_cast<const uint4*>(vc + h * 32 * NB + i);
-                } else if constexpr (NB % 2 == 0) {
-#pragma unroll
-                    for (int i = 0; i < NB; i += 2)
-                        *reinterpret_cast<uint2*>(&vw[h][i]) = *reinterpret_cast<const uint2*>(vc + h * 32 * NB + i);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NB; i++) vw[h][i] = vc[h * 32 * NB + i];
-                }
-            }
-            constexpr uint32_t M8 = 0x80088008u, M8H = 0x80808080u;   // -8 * 2^-24, -8 * 2^-20
-            const uint32_t ones[4] = {M8, M8H, M8, M8H};
-#pragma unroll
-            for (int i = 0; i < NB; i++) {
-                const uint32_t w0 = vw[0][i], w1 = vw[1][i], x0 = w0 >> 8, x1 = w1 >> 8;
-                // rows g: the lower nibbles' dimensions; rows g + 8: the upper ones'
-                const uint32_t a0[4] = {codes_lo<RAW>(w0), codes_hi<RAW>(w0), codes_lo<RAW>(w1), codes_hi<RAW>(w1)};
-                const uint32_t a1[4] = {codes_lo<RAW>(x0), codes_hi<RAW>(x0), codes_lo<RAW>(x1), codes_hi<RAW>(x1)};
+            for (int u = 0; u < U; u++) {
+                const uint8_t* gr = step + u * GB;
+                // ---- p in pieces, transposed: lane (g, c) gets row g's tokens 2c, 2c + 1 of each half
+                uint32_t ph[NT][PC][2];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    uint32_t pb[PC][2];
+                    float p[4];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const __half2 d = as_h2(vd[h][i]), p0 = as_h2(ph[n][0][h]);
-                        __half2 hi = __hmul2(p0, d);
-                        if constexpr (PC == 2) {
-                            // what the product lost, and the lower piece's
-                            __half2 lo = __hfma2(as_h2(ph[n][1][h]), d, __hfma2(p0, d, __hneg2(hi)));
-                            if (mend) lo = as_u32(p0) & 0x7fffu ? lo : __halves2half2(__float2half_rn(0.0f), __high2half(lo));
-                            if (mend) lo = as_u32(p0) & 0x7fff0000u ? lo : __halves2half2(__low2half(lo), __float2half_rn(0.0f));
-                            pb[1][h] = as_u32(lo);
-                        }
-                        if (mend) {
-                            if (!(as_u32(p0) & 0x7fffu)) hi = __halves2half2(__float2half_rn(0.0f), __high2half(hi));
-                            if (!(as_u32(p0) & 0x7fff0000u)) hi = __halves2half2(__low2half(hi), __float2half_rn(0.0f));
-                        }
-                        pb[0][h] = as_u32(hi);
+                    for (int x = 0; x < 4; x++) {
+                        p[x] = ex2(t[u][n][x]);
+                        l[n][x & 1] += p[x];
                     }
 #pragma unroll
-                    for (int p = 0; p < PC; p++) {
-                        mma16816(o[n][2 * i], a0, pb[p][0], pb[p][1]);
-                        mma16816(o[n][2 * i + 1], a1, pb[p][0], pb[p][1]);
-                        if constexpr (RAW) mma16816(oc[n][i], ones, pb[p][0], pb[p][1]);
+                    for (int h = 0; h < 2; h++) {
+                        const __half2 hi = __floats2half2_rn(p[2 * h], p[2 * h + 1]);
+                        ph[n][0][h] = transpose8(as_u32(hi));
+                        if constexpr (PC == 2)
+                            ph[n][1][h] = transpose8(
+                                as_u32(__floats2half2_rn(p[2 * h] - __low2float(hi), p[2 * h + 1] - __high2float(hi))));
+                    }
+                }
+
+                // ---- O += (p d) V
+                uint32_t vd[2][NB], vw[2][NB];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    load_words<NB>(vd[h], gr + 17 * HD + (h * 4 + c) * NB * 4);
+                    load_words<NB>(vw[h], gr + 8 * HD + (h * 32 + lane) * NB * 4);
+#pragma unroll
+                    for (int i = 0; i < NB; i++) vd[h][i] = as_u32(__hmul2(as_h2(vd[h][i]), vmul));
+                }
+                // a block held as NaN may lie behind a row's limit, where it must not meet even a
+                // probability of 0
+                auto keep = [&](int n, int h, uint32_t d) {
+                    if (!mend) return d;
+                    const int seen = lim_g[n] - (t0 + 16 * u + 8 * h + 2 * c);
+                    return seen >= 2 ? d : seen == 1 ? d & 0xffffu : 0u;
+                };
+                if constexpr (NT == 1) {
+                    if (mend)
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int i = 0; i < NB; i++) vd[h][i] = keep(0, h, vd[h][i]);
+                }
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    const uint32_t w0 = vw[0][i], w1 = vw[1][i], x0 = w0 >> 8, x1 = w1 >> 8;
+                    // rows g: the lower nibbles' dimensions; rows g + 8: the upper ones'
+                    const uint32_t a0[4] = {codes_lo<false>(w0, k1024), codes_hi<false>(w0, k1024),
+                                            codes_lo<false>(w1, k1024), codes_hi<false>(w1, k1024)};
+                    const uint32_t a1[4] = {codes_lo<false>(x0, k1024), codes_hi<false>(x0, k1024),
+                                            codes_lo<false>(x1, k1024), codes_hi<false>(x1, k1024)};
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        uint32_t pb[PC][2];
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const __half2 d = as_h2(NT == 1 ? vd[h][i] : keep(n, h, vd[h][i])), p0 = as_h2(ph[n][0][h]);
+                            const __half2 hi = __hmul2(p0, d);
+                            pb[0][h] = as_u32(hi);
+                            // what the product lost, and the lower piece's
+                            if constexpr (PC == 2)
+                                pb[1][h] = as_u32(__hfma2(as_h2(ph[n][1][h]), d, __hfma2(p0, d, __hneg2(hi))));
+                        }
+#pragma unroll
+                        for (int p = 0; p < PC; p++) {
+                            mma16816(o[n][2 * i], a0, pb[p][0], pb[p][1]);
+                            mma16816(o[n][2 * i + 1], a1, pb[p][0], pb[p][1]);
+                        }
                     }
                 }
             }
@@ -585,7 +649,7 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS) k_kvq_attn(AttnKvqArgs a) {
         constexpr int PR = HD + 4;   // floats per row: O, then m and l
         float* js = reinterpret_cast<float*>(sm) + wid * ROWS * PR;
         __syncthreads();
-        const float back = scalbnf(1.0f, min(max((RAW ? 24 : 0) - 6 + vexp, -126), 127));   // out of the units of p, the codes and vexp
+        const float back = scalbnf(1.0f, vexp - 6);   // out of the units of p and vexp
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -598,9 +662,8 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS) k_kvq_attn(AttnKvqArgs a) {
                 for (int i = 0; i < NB; i++)
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
-                        row[32 * i + 16 * t + g] = (o[n][2 * i + t][k] + oc[n][RAW ? i : 0][k]) * back;
-                        row[32 * i + 16 * t + 8 + g] =
-                            (o[n][2 * i + t][k + 2] + oc[n][RAW ? i : 0][k + 2]) * (RAW ? 0.0625f : 1.0f) * back;
+                        row[32 * i + 16 * t + g] = o[n][2 * i + t][k] * back;
+                        row[32 * i + 16 * t + 8 + g] = o[n][2 * i + t][k + 2] * back;
                     }
                 if (g == 0) {
                     row[HD] = m[n][k];
@@ -651,61 +714,153 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS) k_kvq_attn(AttnKvqArgs a) {
     }
 }
 
-// One CTA per (worker, query row of an item): where the worker's second slot begins an item,
-// the parts of the following workers are added to it up to the item's last.
+// Adding up the parts of an item: the second slot of the worker w that begins it, then the
+// first slots of w + 1, ... up to the item's last.
+constexpr int JT = 256, JW = JT / 32;
+
+template <int HD, int ROWS>
+__device__ __forceinline__ const float* join_part(const AttnKvqArgs& a, int w, int i, int r) {
+    return a.slots + ((size_t)(i == 0 ? 2 * w + 1 : 2 * (w + i)) * ROWS + r) * (HD + 4);
+}
+
+// Where row r of the item that begins with head h (kind, token, head, rows) belongs.
+template <typename T>
+__device__ __forceinline__ T* join_out(const AttnKvqArgs& a, const int4& h, int r) {
+    const int rho = h.z % a.R + r;   // query row counted from the first token of the tile
+    return reinterpret_cast<T*>(a.out) + (size_t)(h.y + rho / a.R) * a.os +
+           (size_t)(h.z / a.R * a.R + rho % a.R) * a.c.hd;
+}
+
+// Up to a few parts per item: a CTA per worker, a warp per query row.
 template <int DT, int NB, int NT>
-__global__ void __launch_bounds__(128) k_kvq_join(AttnKvqArgs a) {
+__global__ void __launch_bounds__(JT) k_kvq_join(AttnKvqArgs a) {
     using T = typename Elem<DT>::T;
-    constexpr int HD = 32 * NB, ROWS = 8 * NT, PR = HD + 4;
-    __shared__ float s_o[4][HD], s_l[4], s_m[4];
-    __shared__ int s_n;
-    const int w = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    constexpr int HD = 32 * NB, ROWS = 8 * NT;
+    const int w = blockIdx.x, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int* h = a.heads + ((size_t)w * 2 + 1) * 4;
-    if (h[0] == SLOT_NONE || r >= h[3]) return;
-    if (wid == 0) {   // workers behind w up to the one with the item's last part
-        int n = 1;
-        for (int x = w + 1; x < a.workers; x += 32) {
-            const int v = x + lane;
-            const int kind = v < a.workers ? a.heads[(size_t)v * 8] : SLOT_LAST;
+    const int4 h = *reinterpret_cast<const int4*>(a.heads + ((size_t)w * 2 + 1) * 4);
+    if (h.x == SLOT_NONE) return;
+    for (int r = threadIdx.x >> 5; r < h.w; r += JW) {
+        float m = -INFINITY, l = 0.0f, o[NB];
+#pragma unroll
+        for (int x = 0; x < NB; x++) o[x] = 0.0f;
+        for (int i0 = 0;; i0 += 32) {   // 32 parts at a time, a lane looking at each
+            const int i = i0 + lane;
+            const bool in = w + i < a.workers;
+            const int kind = i == 0 ? SLOT_MORE : in ? a.heads[(size_t)(w + i) * 8] : SLOT_LAST;
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (in) ml = *reinterpret_cast<const float2*>(join_part<HD, ROWS>(a, w, i, r) + HD);   // of an empty slot, too
             const unsigned last = __ballot_sync(0xffffffffu, kind != SLOT_MORE);
-            if (last) {
-                n += __ffs(last);
-                break;
+            const int n = last ? __ffs(last) : 32;
+            float mn = lane < n ? ml.x : -INFINITY;
+#pragma unroll
+            for (int x = 16; x >= 1; x >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
+            mn = fmaxf(mn, m);
+            const float back = mn == m ? 1.0f : ex2(m - mn);
+            const float f = lane >= n ? 0.0f : ml.x == mn ? 1.0f : ex2(ml.x - mn);
+            m = mn;
+            l = fmaf(l, back, lane < n ? f * ml.y : 0.0f);
+#pragma unroll
+            for (int x = 0; x < NB; x++) o[x] *= back;
+#pragma unroll 4
+            for (int y = 0; y < n; y++) {
+                const float* p = join_part<HD, ROWS>(a, w, i0 + y, r);
+                const float fy = __shfl_sync(0xffffffffu, f, y);
+#pragma unroll
+                for (int x = 0; x < NB; x++) o[x] = fmaf(fy, p[32 * x + lane], o[x]);
             }
-            n += 32;
+            if (last) break;
         }
-        if (lane == 0) s_n = n;
+#pragma unroll
+        for (int x = 16; x >= 1; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+        const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+        T* dst = join_out<T>(a, h, r);
+#pragma unroll
+        for (int x = 0; x < NB; x++) from_f32(o[x] * inv, dst[32 * x + lane]);
+    }
+}
+
+// Few items of many parts: a CTA per (item, query row), its warps dealing out the parts.
+template <int DT, int NB, int NT>
+__global__ void __launch_bounds__(JT) k_kvq_join_wide(AttnKvqArgs a) {
+    using T = typename Elem<DT>::T;
+    constexpr int HD = 32 * NB, ROWS = 8 * NT;
+    __shared__ float s_o[JW][HD], s_l[JW], s_m[JW], s_f[MAX_WORKERS];
+    __shared__ uint8_t s_kind[MAX_WORKERS], s_tail[MAX_WORKERS];
+    __shared__ int s_w, s_n;
+    const int item = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int w = tid; w < a.workers; w += JT) {
+        s_kind[w] = (uint8_t)a.heads[(size_t)w * 8];
+        s_tail[w] = (uint8_t)a.heads[(size_t)w * 8 + 4];
     }
     __syncthreads();
-    const int n = s_n;   // parts: the second slot of w, then the first slots of w + 1, ...
-    auto part = [&](int i) { return a.slots + ((size_t)(i == 0 ? 2 * w + 1 : 2 * (w + i)) * ROWS + r) * PR; };
-    float m = -INFINITY, l = 0.0f, o[NB];
-#pragma unroll
-    for (int i = 0; i < NB; i++) o[i] = 0.0f;
-    for (int i = tid; i < n; i += 128) m = fmaxf(m, part(i)[HD]);
+    if (wid == 0) {   // the item'th worker that begins one, and the parts up to the last
+        int w = -1, seen = 0, n = 0;
+        for (int x = 0; x < a.workers && w < 0; x += 32) {
+            const unsigned begins = __ballot_sync(0xffffffffu, x + lane < a.workers && s_tail[x + lane] != SLOT_NONE);
+            if (seen + __popc(begins) > item) w = x + __fns(begins, 0, item - seen + 1);
+            seen += __popc(begins);
+        }
+        if (w >= 0) {
+            n = 1;
+            for (int x = w + 1;; x += 32) {
+                const unsigned last = __ballot_sync(0xffffffffu, x + lane >= a.workers || s_kind[x + lane] != SLOT_MORE);
+                if (last) {
+                    n += __ffs(last);
+                    break;
+                }
+                n += 32;
+            }
+        }
+        if (lane == 0) s_w = w, s_n = n;
+    }
+    __syncthreads();
+    const int w = s_w, n = min(s_n, a.workers - max(w, 0));
+    if (w < 0) return;
+    const int4 h = *reinterpret_cast<const int4*>(a.heads + ((size_t)w * 2 + 1) * 4);
+    if (r >= h.w) return;
+    float m = -INFINITY;
+    for (int i = tid; i < n; i += JT) m = fmaxf(m, join_part<HD, ROWS>(a, w, i, r)[HD]);
 #pragma unroll
     for (int x = 16; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
     if (lane == 0) s_m[wid] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-#pragma unroll 4
-    for (int i = wid; i < n; i += 4) {
-        const float* p = part(i);
-        const float f = p[HD] == m ? 1.0f : ex2(p[HD] - m);
-        l = fmaf(f, p[HD + 1], l);
+#pragma unroll
+    for (int x = 0; x < JW; x++) m = fmaxf(m, s_m[x]);
+    float l = 0.0f, o[NB];
+    for (int i = tid; i < n; i += JT) {
+        const float2 ml = *reinterpret_cast<const float2*>(join_part<HD, ROWS>(a, w, i, r) + HD);
+        s_f[i] = ml.x == m ? 1.0f : ex2(ml.x - m);
+        l = fmaf(s_f[i], ml.y, l);
+    }
+#pragma unroll
+    for (int x = 0; x < NB; x++) o[x] = 0.0f;
+    __syncthreads();
+#pragma unroll 8
+    for (int i = wid; i < n; i += JW) {
+        const float* p = join_part<HD, ROWS>(a, w, i, r);
+        const float f = s_f[i];
 #pragma unroll
         for (int x = 0; x < NB; x++) o[x] = fmaf(f, p[32 * x + lane], o[x]);
     }
 #pragma unroll
+    for (int x = 16; x >= 1; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+#pragma unroll
     for (int x = 0; x < NB; x++) s_o[wid][32 * x + lane] = o[x];
     if (lane == 0) s_l[wid] = l;
     __syncthreads();
-    l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    l = 0.0f;
+#pragma unroll
+    for (int x = 0; x < JW; x++) l += s_l[x];
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-    const int rho = h[2] % a.R + r;   // query row counted from the first token of the tile
-    T* dst = reinterpret_cast<T*>(a.out) + (size_t)(h[1] + rho / a.R) * a.os + (size_t)(h[2] / a.R * a.R + rho % a.R) * HD;
-    for (int d = tid; d < HD; d += 128) from_f32(((s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d])) * inv, dst[d]);
+    T* dst = join_out<T>(a, h, r);
+    for (int d = tid; d < HD; d += JT) {
+        float x = 0.0f;
+#pragma unroll
+        for (int y = 0; y < JW; y++) x += s_o[y][d];
+        from_f32(x * inv, dst[d]);
+    }
 }
 
 // ---------------------------------------------------------------- launching
@@ -713,10 +868,6 @@ __global__ void __launch_bounds__(128) k_kvq_join(AttnKvqArgs a) {
 // granules dealt out); with more, every warp is a worker of its own.
 constexpr int DEEP_ROWS = 32;
 constexpr int MAX_DEV = 64;
-constexpr int MAX_SMS = 160;
-
-
-constexpr int workers_per_sm(int warps) { return warps > 1 ? 4 : 12; }
 
 // A second tile of 8 query rows takes the same unpacked codes: worth it where there are the
 // rows for it and the registers (fp32 holds q and p twice).
@@ -724,6 +875,7 @@ constexpr bool two_tiles(int dt, int nb) { return nb <= (dt == TGX_F32 ? 3 : 4);
 
 struct Shape {
     int warps, nt, workers;
+    int wide;   // items for the wide join, 0 for the other
 };
 
 // Workers and their row tiles for these bounds; at most `have` workers are resident.
@@ -733,10 +885,12 @@ Shape shape_of(const KvqCache& c, const KvqBatch& b, int R, bool two, int have_o
     sh.warps = rows <= DEEP_ROWS ? DEEP_WARPS : 1;
     sh.nt = rows > 8 && two ? 2 : 1;
     // no more workers than there can be granules for their warps
-    const long long most = (long long)b.B * c.nkv * ((rows + 8 * sh.nt - 1) / (8 * sh.nt)) *
-                           (((long long)b.max_pages * c.pt + 15) / 16);
+    const long long items = (long long)b.B * c.nkv * ((rows + 8 * sh.nt - 1) / (8 * sh.nt));
+    const long long most = items * (((long long)b.max_pages * c.pt + 15) / 16);
     const long long have = sh.warps > 1 ? have_deep : have_one, want = (most + sh.warps - 1) / sh.warps;
     sh.workers = (int)(want < have ? want : have);
+    // many parts per item: 14 us -> see k_kvq_join_wide
+    sh.wide = items * 16 < sh.workers ? (int)items : 0;
     return sh;
 }
 
@@ -767,21 +921,21 @@ int attn_workers(int W) {   // resident CTAs of the device, per kernel and CTA s
 }
 
 template <int DT, int NB, int NT>
-cudaError_t launch_attn_t(AttnKvqArgs a, int W, int workers, cudaStream_t s) {
-    a.workers = workers;
-    k_kvq_attn<DT, NB, NT><<<workers, 32 * W, attn_smem<NB, NT>(W), s>>>(a);
+cudaError_t launch_attn_t(AttnKvqArgs a, const Shape& sh, cudaStream_t s) {
+    a.workers = sh.workers;
+    k_kvq_attn<DT, NB, NT><<<sh.workers, 32 * sh.warps, attn_smem<NB, NT>(sh.warps), s>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(workers, 8 * NT);
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = sh.wide ? dim3(sh.wide, 8 * NT) : dim3(sh.workers);
+    cfg.blockDim = dim3(JT);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_kvq_join<DT, NB, NT>, a);
+    return cudaLaunchKernelEx(&cfg, sh.wide ? k_kvq_join_wide<DT, NB, NT> : k_kvq_join<DT, NB, NT>, a);
 }
 
 template <int DT, int NB>
@@ -795,8 +949,7 @@ cudaError_t launch_attn_nb(AttnKvqArgs a, void* scratch, size_t scratch_bytes, c
     if (scratch_bytes < attn_scratch(sh, a.c.hd)) return cudaErrorInvalidValue;
     a.heads = reinterpret_cast<int*>(scratch);
     a.slots = reinterpret_cast<float*>((uint8_t*)scratch + head_bytes(sh.workers));
-    return nt2 ? launch_attn_t<DT, NB, NT2>(a, sh.warps, sh.workers, s)
-               : launch_attn_t<DT, NB, 1>(a, sh.warps, sh.workers, s);
+    return nt2 ? launch_attn_t<DT, NB, NT2>(a, sh, s) : launch_attn_t<DT, NB, 1>(a, sh, s);
 }
 
 #define TG_NB(DT, F, ...)                     \
@@ -863,7 +1016,7 @@ extern "C" int tgx_kvq_attention(const tgx_kvq_cache* cache, const tgx_kvq_batch
     if (dev.rc != TG_OK || n_tokens == 0) return dev.rc;
     const float sc = (scale > 0.0f ? scale : 1.0f / sqrtf((float)cache->head_dim)) * 1.44269504088896340736f;
     tg::AttnKvqArgs a{tg::kvq_cache(*cache), tg::kvq_batch(*batch), n_tokens, n_heads, n_heads / cache->n_kv_heads, q,
-                      q_stride, out, out_stride, sc, 0, nullptr, nullptr};
+                      q_stride, out, out_stride, sc, 0x64006400u, 0, nullptr, nullptr};
     cudaError_t e = tg::launch_attn(dtype, a, scratch, scratch_bytes, (cudaStream_t)stream);
     return e == cudaSuccess ? TG_OK : tg::serve_fail(TG_ECUDA, fn, cudaGetErrorString(e));
 }

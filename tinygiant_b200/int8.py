@@ -16,17 +16,18 @@ from .paged import dtype_code, on_stream, stream_handle
 
 def _matrix(t, cols, device, name):
     """(pointer, row stride) of a matrix with dense rows."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] != cols or (stride[1] != 1 and cols > 1 and t.numel()):
+        raise ValueError(f"{name}: expected rows of {cols}, dense in a row, got {tuple(shape)} with strides {stride}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if t.dim() != 2 or t.shape[1] != cols or (t.stride(1) != 1 and cols > 1 and t.numel()):
-        raise ValueError(f"{name}: expected rows of {cols}, dense in a row, got {tuple(t.shape)} with strides {t.stride()}")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else cols
+    return t.data_ptr(), stride[0] if shape[0] > 1 else cols
 
 
 def _norm(norm, cols, device):
     if norm is None:
         return None
-    if norm.dtype != torch.float32 or norm.device != device or norm.shape != (cols,) or not norm.is_contiguous():
+    if norm.shape != (cols,) or norm.dtype != torch.float32 or norm.device != device or not norm.is_contiguous():
         raise ValueError(f"norm: expected contiguous float32 [{cols}] on {device}")
     return norm.data_ptr()
 
@@ -83,16 +84,21 @@ class Int8Linear:
         px, sx = _matrix(x, k, dev, "x")
         m = x.shape[0]
         if out is None:
-            out = torch.empty((m, n), dtype=x.dtype, device=dev)
-        po, so = _matrix(out, n, dev, "out")
-        pr, sr = (None, 0) if residual is None else _matrix(residual, n, dev, "residual")
-        if out.dtype != x.dtype or out.shape[0] != m or (
-                residual is not None and (residual.dtype != x.dtype or residual.shape[0] != m)):
-            raise ValueError("out and residual: expected x's type and rows")
+            out = x.new_empty((m, n))
+            po, so = out.data_ptr(), n
+        else:
+            po, so = _matrix(out, n, dev, "out")
+            if out.dtype != x.dtype or out.shape[0] != m:
+                raise ValueError("out: expected x's type and rows")
+        pr, sr = None, 0
+        if residual is not None:
+            pr, sr = _matrix(residual, n, dev, "residual")
+            if residual.dtype != x.dtype or residual.shape[0] != m:
+                raise ValueError("residual: expected x's type and rows")
         if not m:
             return out
         size = self.lib.tgx_i8_matmul_scratch_bytes(m, n, k)
-        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+        scratch = self.codes.new_empty(size)
         check(self.lib.tgx_i8_matmul(dtype_code(x), px, sx, m, k, _norm(norm, k, dev), eps, self.codes.data_ptr(),
                                      self.scales.data_ptr(), n, pr, sr, po, so, scratch.data_ptr(), size,
                                      stream_handle(dev)), self.lib)

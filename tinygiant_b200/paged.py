@@ -29,9 +29,14 @@ def dtype_code(t) -> int:
     return code
 
 
+# The cudaStream_t of a device's current stream, by the device's index; torch's own accessor
+# without the Stream object around it, a tenth of current_stream()'s time.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def stream_handle(device) -> int:
     """The cudaStream_t of the device's current stream."""
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index)
 
 
 def on_stream(stream, device):
@@ -45,23 +50,24 @@ def on_stream(stream, device):
 def rows_of(t, heads: int, head_dim: int, device, name: str):
     """(pointer, row stride) of token rows [T][heads][head_dim] or [T][heads * head_dim]: each
     row dense, rows any distance apart."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3:
+        ok = shape[1] == heads and shape[2] == head_dim and stride[2] == 1 and (stride[1] == head_dim or heads == 1)
+    else:
+        ok = len(shape) == 2 and shape[1] == heads * head_dim and stride[1] == 1
+    if not ok and t.numel():
+        raise ValueError(f"{name}: expected rows of {heads} heads of {head_dim}, dense in a row, got {tuple(shape)} "
+                         f"with strides {stride}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the cache on {device}")
-    if t.dim() == 3:
-        ok = t.shape[1] == heads and t.shape[2] == head_dim and (t.stride(2) == 1) and (t.stride(1) == head_dim or heads == 1)
-    else:
-        ok = t.dim() == 2 and t.shape[1] == heads * head_dim and t.stride(1) == 1
-    if not ok and t.numel():
-        raise ValueError(f"{name}: expected rows of {heads} heads of {head_dim}, dense in a row, got {tuple(t.shape)} "
-                         f"with strides {t.stride()}")
     # the stride of a single row says nothing: any value may stand there
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else heads * head_dim
+    return t.data_ptr(), stride[0] if shape[0] > 1 else heads * head_dim
 
 
 def _f32(t, shape, device, name):
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.device != device or not t.is_contiguous() or tuple(t.shape) != shape:
+    if t.shape != shape or t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name}: expected contiguous float32 {shape} on {device}")
     return t.data_ptr()
 
@@ -153,7 +159,7 @@ class PagedKV4:
             if q.dtype != k.dtype or q.shape[0] != t:
                 raise ValueError("q and k differ in type or rows")
             if q_out is None:
-                q_out = torch.empty((t, heads, hd), dtype=q.dtype, device=dev)
+                q_out = q.new_empty((t, heads, hd))
             elif q_out.dtype != q.dtype or q_out.device != dev or not q_out.is_contiguous() or \
                     q_out.numel() != t * heads * hd:
                 raise ValueError("q_out: expected contiguous rows like q")
@@ -181,7 +187,7 @@ class PagedKV4:
                 return self.read(batch, n_tokens)
         shape = (n_tokens, self.n_kv_heads, self.head_dim)
         k = torch.empty(shape, dtype=torch.float32, device=self.device)
-        v = torch.empty(shape, dtype=torch.float32, device=self.device)
+        v = torch.empty_like(k)
         if n_tokens:
             check(self.lib.tgx_kvq_read(self.ref, self._batch(batch), n_tokens, k.data_ptr(), v.data_ptr(),
                                         stream_handle(self.device)), self.lib)
@@ -198,15 +204,17 @@ class PagedKV4:
         qp, qs = rows_of(q, heads, hd, dev, "q")
         t = q.shape[0]
         if out is None:
-            out = torch.empty((t, heads, hd), dtype=q.dtype, device=dev)
-        op, os = rows_of(out, heads, hd, dev, "out")
-        if out.dtype != q.dtype or out.shape[0] != t:
-            raise ValueError("out: expected rows like q")
+            out = q.new_empty((t, heads, hd))
+            op, os = out.data_ptr(), heads * hd
+        else:
+            op, os = rows_of(out, heads, hd, dev, "out")
+            if out.dtype != q.dtype or out.shape[0] != t:
+                raise ValueError("out: expected rows like q")
         bref = self._batch(batch)
         if not t:
             return out
         n = self.lib.tgx_kvq_attention_scratch_bytes(self.ref, bref, t, heads)
-        scratch = torch.empty(max(n, 256), dtype=torch.uint8, device=dev)
+        scratch = self.pages.new_empty(max(n, 256))
         check(self.lib.tgx_kvq_attention(self.ref, bref, dtype_code(q), t, qp, qs, heads, op, os, scale,
                                          scratch.data_ptr(), n, stream_handle(dev)), self.lib)
         return out
