@@ -25,10 +25,10 @@
 // 2^-17 of sum |q| 16 d: enough for a score behind 16-bit inputs, too coarse for fp32, and for
 // V, where sum 8 p d would have to cancel.)
 //
-// Work: an item is (sequence, kv head, tile of 8 * NT query rows), its units the granules
-// of 16 tokens (18 * HD contiguous bytes).  All items' units in one line are cut into equal
-// parts, one per worker (a CTA of W warps), whatever the lengths: a worker walks the items of
-// its part.  Each of its warps takes every W-th granule, through a ring of its own that
+// Work: an item is (sequence, kv head, tile of 8 * NT query rows) over the sequence's granules
+// of 16 tokens (18 * HD contiguous bytes).  A worker is a CTA of W warps.  All items in one line are
+// cut into one part per worker, whatever the lengths, and a worker walks the items of its part;
+// few items are each cut into equal parts, a worker each.  Each of its warps takes every W-th pair of granules, through a ring of its own that
 // cp.async keeps STAGES deep, and the W results meet in shared memory.  An item that lies in
 // one part is finished there; the others' parts go to scratch and k_kvq_join adds them in
 // order, so results repeat exactly.
@@ -64,6 +64,10 @@ struct AttnKvqArgs {
     float* slots;       // [workers][2] partial results: m, l [rows], O [rows][HD]
     int* heads;         // [workers][2][4] what a slot holds: kind, token row base, kv head, query rows
 };
+
+// What beginning an item costs beside its granules, in a warp's granules: about 5 us measured
+// (queries, first copies, joining the warps), against 0.6 us for a granule.
+constexpr int OPEN_UNITS = 8;
 
 // Slot kinds: nothing; a part that its item goes on behind; the item's last part.
 constexpr int MAX_SMS = 160;
@@ -188,11 +192,36 @@ constexpr int min_ctas(int nb, int nt) { return nb <= 3 && nt == 1 ? 4 : nb * nt
 constexpr int STAGES = 3;
 constexpr int U = 2;   // granules of a stage, and of a step of the loop
 
-// Shared memory of a CTA of W warps: the rings, which the joining of the warps reuses.
+// Shared memory of a CTA of W warps: the rings, which the joining of the warps reuses, then
+// the query rows' operands, factors and limits.
 template <int NB, int NT>
-constexpr int attn_smem(int W) {
+constexpr int attn_ring(int W) {
     const int ring = W * STAGES * U * 18 * 32 * NB, join = W * 8 * NT * (32 * NB + 4) * 4;
     return ring > join ? ring : join;
+}
+template <int NB, int NT>
+constexpr int attn_smem(int W) {
+    return attn_ring<NB, NT>(W) + NT * 2 * NB * 512 + 8 * NT * (NB + 2) * 4;
+}
+
+// Exclusive prefix of v over the CTA's threads; `total` gets the sum.
+__device__ __forceinline__ long long block_sum(long long v, long long& total, long long* s_scan, int W) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    long long incl = v, before = 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_scan[wid] = incl;
+    __syncthreads();
+    total = 0;
+    for (int i = 0; i < W; i++) {
+        if (i < wid) before += s_scan[i];
+        total += s_scan[i];
+    }
+    __syncthreads();
+    return before + incl - v;
 }
 
 template <int DT, int NB, int NT>
@@ -202,81 +231,121 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
     constexpr int PC = DT == TGX_F32 ? 2 : 1;    // fp16 pieces of q and of p * d
     constexpr bool RAW = PC == 1;                // K's codes as subnormals
     extern __shared__ __align__(16) uint8_t sm[];
-    __shared__ long long s_scan[8];
+    __shared__ long long s_scan[DEEP_WARPS];
     __shared__ long long s_base;
     __shared__ int s_seq;
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, W = blockDim.x >> 5;
     const int g = lane >> 2, c = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    // ---- the plan: every worker adds up all sequences' units and finds where its part begins.
-    // Thread t owns sequences [t * per, ...), so a prefix over the threads is one over them.
-    const int per = (a.b.B + (int)blockDim.x - 1) / (int)blockDim.x;
-    long long mine = 0;
+    // ---- the plan, made by every worker for itself.  Thread t owns sequences [t * per, ...), so
+    // a prefix over the threads is one over them.  Units: granules, and OPEN for each item, what
+    // beginning another item costs.
+    const int per = (a.b.B + (int)blockDim.x - 1) / (int)blockDim.x, w = blockIdx.x;
+    const int OPEN = OPEN_UNITS * W;
+    long long mine = 0, grans = 0, before, total, total_grans, items = 0;
     for (int i = 0; i < per; i++) {
         const int b = tid * per + i;
         if (b < a.b.B) {
             const SeqInfo s = seq_info(a, b, ROWS);
-            mine += (long long)s.tiles * s.grans * a.c.nkv;
-            if (blockIdx.x == 0 && (long long)a.b.kv_lens[b] > (long long)a.b.max_pages * a.c.pt)
-                kvq_flag(a.b, TGX_KVQ_BAD_LENGTH);
-            if (blockIdx.x == 0 && (long long)a.b.q_start[b + 1] - a.b.q_start[b] > a.b.max_new)
-                kvq_flag(a.b, TGX_KVQ_BAD_NEW);
+            const long long n = (long long)s.tiles * a.c.nkv;
+            mine += n;
+            grans += n * s.grans;
+            if (w == 0 && (long long)a.b.kv_lens[b] > (long long)a.b.max_pages * a.c.pt) kvq_flag(a.b, TGX_KVQ_BAD_LENGTH);
+            if (w == 0 && (long long)a.b.q_start[b + 1] - a.b.q_start[b] > a.b.max_new) kvq_flag(a.b, TGX_KVQ_BAD_NEW);
         }
     }
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 31) s_scan[wid] = incl;
-    __syncthreads();
-    long long before = 0, total = 0;
-    for (int i = 0; i < W; i++) {
-        if (i < wid) before += s_scan[i];
-        total += s_scan[i];
-    }
-    // at least one step per warp of a worker: short work goes to fewer workers
-    const long long used = max(1ll, min((long long)a.workers, quotient(total + U * W - 1, U * W)));
-    const long long w = blockIdx.x;
-    const long long share = quotient(total, used), more = total - share * used;   // `more` workers have one unit more
-    long long u = w < used ? share * w + min(w, more) : total;
-    const long long u_end = w < used ? u + share + (w < more ? 1 : 0) : total;
-    if (tid < 2) {   // no slots yet
-        a.heads[((size_t)w * 2 + tid) * 4] = SLOT_NONE;
-    }
-    if (u >= u_end) return;
-    if (u >= before + incl - mine && u < before + incl) {
-        long long x = before + incl - mine;
-        int b = tid * per;
-        for (;; b++) {
-            const SeqInfo s = seq_info(a, b, ROWS);
-            const long long n = (long long)s.tiles * s.grans * a.c.nkv;
-            if (u < x + n) break;
-            x += n;
+    if (tid < 2) a.heads[((size_t)w * 2 + tid) * 4] = SLOT_NONE;   // no slots yet
+    block_sum(mine, items, s_scan, W);
+    block_sum(grans, total_grans, s_scan, W);
+    int b, item, g0, g1;            // the piece at hand: sequence, item in it, granules
+    long long u = 0, u_end = 0, base = 0;
+    // One line of all items cut into equal parts, or each item in parts of its own, of at most
+    // `quota` granules, where that is no longer than a part of the line and a second beginning in it.
+    const int step = U * W;
+    const long long room = a.workers - items;
+    const long long quota = room > 0 ? max(1ll, quotient(quotient(total_grans, room) + step, step)) * step : 0;
+    const bool few = room > 0 && quota <= quotient(total_grans + items * OPEN, a.workers) + OPEN;
+    if (few) {
+        auto parts = [&](const SeqInfo& s) { return (int)quotient(s.grans + quota - 1, quota); };
+        mine = 0;
+        for (int i = 0; i < per; i++) {
+            const int b = tid * per + i;
+            if (b < a.b.B) {
+                const SeqInfo s = seq_info(a, b, ROWS);
+                mine += (long long)s.tiles * a.c.nkv * parts(s);
+            }
         }
-        s_seq = b;
-        s_base = x;
+        before = block_sum(mine, total, s_scan, W);
+        if (w >= total) return;
+        if (w >= before && w < before + mine) {
+            long long x = before;
+            int b = tid * per;
+            for (;; b++) {
+                const SeqInfo s = seq_info(a, b, ROWS);
+                const long long n = (long long)s.tiles * a.c.nkv * parts(s);
+                if (w < x + n) break;
+                x += n;
+            }
+            s_seq = b;
+            s_base = x;
+        }
+        __syncthreads();
+        b = s_seq;
+        const SeqInfo s = seq_info(a, b, ROWS);
+        const int n = parts(s), part = (int)(w - s_base) % n;
+        item = (int)(w - s_base) / n;
+        g0 = (int)((long long)s.grans * part / n);
+        g1 = (int)((long long)s.grans * (part + 1) / n);
+    } else {   // one line, cut into equal parts
+        mine = grans + mine * OPEN;
+        before = block_sum(mine, total, s_scan, W);
+        const long long share = quotient(total, a.workers), more = total - share * a.workers;   // one unit more
+        u = share * w + min((long long)w, more);
+        u_end = u + share + (w < more ? 1 : 0);
+        if (u >= u_end) return;
+        if (u >= before && u < before + mine) {
+            long long x = before;
+            int b = tid * per;
+            for (;; b++) {
+                const SeqInfo s = seq_info(a, b, ROWS);
+                const long long n = (long long)s.tiles * a.c.nkv * (s.grans + OPEN);
+                if (u < x + n) break;
+                x += n;
+            }
+            s_seq = b;
+            s_base = x;
+        }
+        __syncthreads();
+        b = s_seq;
+        base = s_base;   // units in front of sequence b
     }
-    __syncthreads();
-    int b = s_seq;
-    long long base = s_base;   // units in front of sequence b
 
     uint8_t* ring = sm + wid * ST * U * GB;
+    uint32_t* s_q = reinterpret_cast<uint32_t*>(sm + attn_ring<NB, NT>(W));   // q's operands, [tile][piece][NB][lane][4]
+    float* s_corr = reinterpret_cast<float*>(s_q + NT * PC * KS * 64);        // [row][NB]
+    float* s_fac = s_corr + ROWS * NB;
+    int* s_lim = reinterpret_cast<int*>(s_fac + ROWS);
     const uint32_t k1024 = a.k1024;
-    while (u < u_end) {
+    do {
         const SeqInfo si = seq_info(a, b, ROWS);
-        const long long units = (long long)si.tiles * si.grans * a.c.nkv;
-        if (u >= base + units) {
-            base += units;
-            b++;
-            continue;
+        if (!few) {
+            const int each = si.grans + OPEN;
+            const long long units = (long long)si.tiles * a.c.nkv * each;
+            if (u >= base + units) {
+                base += units;
+                b++;
+                continue;
+            }
+            item = (int)quotient(u - base, each);
+            const int x = (int)(u - base - (long long)item * each);
+            const int y = (int)min((long long)each, x + (u_end - u));
+            u += y - x;
+            g0 = max(0, x - OPEN);
+            g1 = y - OPEN;
+            if (g1 <= g0) continue;   // units of its beginning only: the next worker begins it
         }
-        const int item = (int)quotient(u - base, si.grans), g0 = (int)(u - base - (long long)item * si.grans);
         const int rt = item / a.c.nkv, j = item % a.c.nkv;   // kv heads innermost
-        const int g1 = (int)min((long long)si.grans, g0 + (u_end - u));
-        u += g1 - g0;
         const int row0 = rt * ROWS, nrows = min(ROWS, si.n * a.R - row0);   // query rows of the item
 
         // rows that new token i attends to: those below its limit
@@ -334,67 +403,76 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
         for (int k = 0; k < ST - 1; k++) issue(k);
 
         // ---- the query rows as B operands: lane (g, c) holds row g's dimensions 16s + 2c, + 1
-        // and + 8, and the rows' factors, limits and offsets for the columns 2c, 2c + 1
+        // and + 8, and the rows' factors, limits and offsets for the columns 2c, 2c + 1.  A warp
+        // makes every W-th row's, for all; lane l takes the pairs of dimensions 2l + 64x, + 1.
+        for (int r = wid; r < ROWS; r += W) {
+            const bool ok = r < nrows;
+            const int rho = row0 + r;
+            const T* src = reinterpret_cast<const T*>(a.q) + (size_t)(si.s0 + (ok ? rho / a.R : 0)) * a.qs +
+                           (size_t)(j * a.R + (ok ? rho % a.R : 0)) * HD;
+            constexpr int NP = (NB + 1) / 2;
+            float2 x[NP];
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                x[i] = make_float2(0.0f, 0.0f);
+                if (ok && (NB % 2 == 0 || 64 * i + 2 * lane < HD)) x[i] = load2(src + 64 * i + 2 * lane);
+                top = fmaxf(top, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+            }
+#pragma unroll
+            for (int y = 16; y >= 1; y >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
+            // 2^-e: top into 2^13 .. 2^14, from its exponent field (e down to -113 for tiny ones).  The
+            // factor is two powers of two: e reaches beyond fp32's exponents
+            const int field = (int)(__float_as_uint(top) >> 23);
+            const int e = field == 255 || top == 0.0f ? 0 : max(field - 127, -100) - 13, half = e / 2;
+            const float up1 = __uint_as_float((uint32_t)(127 - half) << 23), up2 = __uint_as_float((uint32_t)(127 - (e - half)) << 23);
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const int d = 64 * i + 2 * lane, s = d / 16, h = d / 8 % 2, cc = d / 2 % 4, word = 2 * s + h;
+                const float y0 = x[i].x * up1 * up2, y1 = x[i].y * up1 * up2;
+                const float m = RAW && h ? 0.0625f : 1.0f;   // the upper nibbles' codes count 16 times
+                const __half2 hi = __floats2half2_rn(y0 * m, y1 * m);
+                uint32_t* to = s_q + ((r / 8 * PC) * NB + word / 4) * 128 + (r % 8 * 4 + cc) * 4 + word % 4;
+                float sum = y0 + y1;
+#pragma unroll
+                for (int y = 8; y >= 1; y >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, y);
+                if (NB % 2 == 0 || d < HD) {
+                    to[0] = as_u32(hi);
+                    if constexpr (PC == 2)
+                        to[NB * 128] = as_u32(__floats2half2_rn(y0 * m - __low2float(hi), y1 * m - __high2float(hi)));
+                    if (lane % 16 == 0) s_corr[r * NB + d / 32] = sum * (-8.0f * 0x1p-24f);
+                }
+            }
+            if (lane == 0) {
+                s_fac[r] = a.scale * (RAW ? 0x1p24f : 1.0f) * __uint_as_float((uint32_t)(127 + half) << 23) *
+                           __uint_as_float((uint32_t)(127 + e - half) << 23);
+                s_lim[r] = ok ? limit(rho / a.R) : 0x7fffffff;   // rows beyond the item: any scores will do
+            }
+        }
+        __syncthreads();
         uint32_t qf[NT][PC][KS][2];
         float corr[NT][NB][4], fac[NT][2];
         int lim[NT][2], lim_g[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const int r = 8 * n + g;
-            const bool ok = r < nrows;
-            const int rho = row0 + r;
-            const T* src = reinterpret_cast<const T*>(a.q) + (size_t)(si.s0 + (ok ? rho / a.R : 0)) * a.qs +
-                           (size_t)(j * a.R + (ok ? rho % a.R : 0)) * HD;
-            float x[KS][4], top = 0.0f;
 #pragma unroll
-            for (int s = 0; s < KS; s++)
+            for (int p = 0; p < PC; p++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float2 y = ok ? load2(src + 16 * s + 8 * h + 2 * c) : make_float2(0.0f, 0.0f);
-                    x[s][2 * h] = y.x;
-                    x[s][2 * h + 1] = y.y;
-                    top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
+                for (int i = 0; i < NB; i++) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(s_q + ((n * PC + p) * NB + i) * 128 + lane * 4);
+                    qf[n][p][2 * i][0] = v.x;
+                    qf[n][p][2 * i][1] = v.y;
+                    qf[n][p][2 * i + 1][0] = v.z;
+                    qf[n][p][2 * i + 1][1] = v.w;
                 }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // 2^-e: top into 2^13 .. 2^14 (in two factors: e reaches beyond fp32's exponents)
-            int e = top > 0.0f && top <= 3.4e38f ? ilogbf(top) - 13 : 0;
-            e = max(e, -110);
-            const float up1 = scalbnf(1.0f, -(e / 2)), up2 = scalbnf(1.0f, -(e - e / 2));
-            float sums[NB];
-#pragma unroll
-            for (int i = 0; i < NB; i++) sums[i] = 0.0f;
-#pragma unroll
-            for (int s = 0; s < KS; s++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float y0 = x[s][2 * h] * up1 * up2, y1 = x[s][2 * h + 1] * up1 * up2;
-                    sums[s >> 1] += y0 + y1;
-                    const float m = RAW && h ? 0.0625f : 1.0f;   // the upper nibbles' codes count 16 times
-                    const __half2 hi = __floats2half2_rn(y0 * m, y1 * m);
-                    qf[n][0][s][h] = as_u32(hi);
-                    if constexpr (PC == 2)
-                        qf[n][1][s][h] =
-                            as_u32(__floats2half2_rn(y0 * m - __low2float(hi), y1 * m - __high2float(hi)));
-                }
-            float f = a.scale * (RAW ? 0x1p24f : 1.0f);
-            f = scalbnf(f, e);
-            const int l = ok ? limit(rho / a.R) : 0x7fffffff;   // rows beyond the item: any scores will do
-            lim_g[n] = l;
+            lim_g[n] = s_lim[8 * n + g];
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                fac[n][k] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + k));
-                lim[n][k] = __shfl_sync(0xffffffffu, l, 4 * (2 * c + k));
-            }
+                fac[n][k] = s_fac[8 * n + 2 * c + k];
+                lim[n][k] = s_lim[8 * n + 2 * c + k];
 #pragma unroll
-            for (int i = 0; i < NB; i++) {
-                float t = sums[i];
-                t += __shfl_xor_sync(0xffffffffu, t, 1);
-                t += __shfl_xor_sync(0xffffffffu, t, 2);
-                t = RAW ? t * (-8.0f * 0x1p-24f) : 0.0f;
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    corr[n][i][k] = __shfl_sync(0xffffffffu, t, 4 * (2 * c + k));
+                for (int i = 0; i < NB; i++) {
+                    corr[n][i][k] = s_corr[(8 * n + 2 * c + k) * NB + i];
                     // a register of its own: the accumulator's four are read together
                     asm volatile("mov.f32 %0, %1;" : "=f"(corr[n][i][k + 2]) : "f"(corr[n][i][k]));
                 }
@@ -711,7 +789,7 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
             h[3] = nrows;
         }
         __syncthreads();
-    }
+    } while (u < u_end);
 }
 
 // Adding up the parts of an item: the second slot of the worker w that begins it, then the
