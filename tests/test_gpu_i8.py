@@ -84,7 +84,8 @@ def check(x, lin, norm=None, residual=None, eps=1e-5, **kw):
 
 SHAPES = [(1, 1, 1), (1, 5120, 2048), (2, 37, 155), (3, 129, 48), (8, 512, 4096), (9, 1000, 1000), (16, 257, 2049),
           (17, 64, 16), (31, 2048, 768), (64, 300, 4096), (65, 1025, 333), (128, 128, 128), (129, 255, 640),
-          (200, 777, 1999), (513, 513, 513), (1, 33, 131072), (300, 40, 7168)]
+          (200, 777, 1999), (513, 513, 513), (1, 33, 131072), (300, 40, 7168), (96, 2048, 4096),
+          (90, 500, 8000), (250, 1000, 2048), (700, 2000, 300)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])

@@ -111,8 +111,8 @@ __global__ void __launch_bounds__(QT) k_i8_rows(QuantArgs a) {
 // and few tokens cost few columns.  Operands come by TMA, K in steps of 128 bytes, 128-byte
 // swizzle, into a ring of stages; rows and bytes beyond the matrices are filled with zeros.
 //
-// Warps 0 .. 3 are the epilogue (TMEM lanes 32 w ..), warp 4 issues the copies, warp 5 the
-// MMAs.  A CTA walks its tiles; with two accumulators the epilogue of one runs behind the
+// Warps 0 .. 7 are the epilogue (TMEM lanes 32 (w % 4) .., every second 16 columns), warp 8
+// issues the copies, warp 9 the MMAs.  A CTA walks its tiles; with two accumulators the epilogue of one runs behind the
 // MMAs of the next.  Where there are fewer tiles than SMs, K is split over the CTAs of a
 // cluster: each puts its int32 sums into its own shared memory, and every CTA adds up and
 // finishes every splits-th column, exactly, whatever the split.
@@ -137,7 +137,9 @@ struct MatArgs {
 constexpr int TM = 128;           // channels per tile
 constexpr int KB = 128;           // bytes of K per stage
 constexpr int MAX_STAGES = 12;
-constexpr int GT = 192;           // threads
+constexpr int MAX_SPLITS = 4;     // larger clusters of one CTA per SM wait for room in a GPC: 8 took 20 us where 4 take 15
+constexpr int EW = 8;             // epilogue warps
+constexpr int GT = 32 * (EW + 2); // threads
 constexpr long long WAIT_CYCLES = 2000000000ll;   // about a second
 
 __device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -214,6 +216,7 @@ __global__ void __launch_bounds__(GT, 1)
     __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_free[2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
+    __shared__ __align__(16) float s_sa[2][256];   // the tokens' scales of a tile
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     volatile int* failed = &s_failed;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -231,12 +234,12 @@ __global__ void __launch_bounds__(GT, 1)
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_free[i], 128);
+            mbar_init(&acc_free[i], 32 * EW);
         }
         s_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;");
     }
-    if (warp == 5) {
+    if (warp == EW + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&s_tmem)), "r"(cols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -245,60 +248,69 @@ __global__ void __launch_bounds__(GT, 1)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
 
-    if (warp == 4) {
+    if (warp == EW) {
         if (lane == 0) {
             // x is the quantiser's: only weights may be fetched before it has finished
-            const int n_mine = first < tiles ? (tiles - first + stride - 1) / stride : 0;
-            const int ahead = min(g.stages, n_mine * (k1 - k0));
-            for (int f = 0; f < ahead; f++) {
-                const int tile = first + f / (k1 - k0) * stride, k = k0 + f % (k1 - k0);
+            const int steps = k1 - k0, n_mine = first < tiles ? (tiles - first + stride - 1) / stride : 0;
+            const int ahead = min(g.stages, n_mine * steps);
+            for (int f = 0, k = 0, tile = first; f < ahead; f++) {
                 mbar_expect(&full[f], stage_bytes);
-                tma_load(sm + f * stage_bytes, &mw, k * KB, tile % nt * TM, &full[f]);
+                tma_load(sm + f * stage_bytes, &mw, (k0 + k) * KB, tile % nt * TM, &full[f]);
+                if (++k == steps) k = 0, tile += stride;
             }
             asm volatile("griddepcontrol.wait;" ::: "memory");
-            int f = 0, issued = 0;
+            // one thread feeds the ring: stage and phase are counted, not divided out
+            int issued = 0, s = 0;
+            uint32_t phase = 1;   // of `empty`: a fresh barrier's wait for it passes
             bool ok = true;
-            for (int tile = first; tile < tiles && ok; tile += stride)
-                for (int k = k0; k < k1 && ok; k++, f++) {
-                    const int s = f % g.stages;
+            for (int tile = first; tile < tiles && ok; tile += stride) {
+                const int y = tile % nt * TM, my = tile / nt * g.tn;
+                for (int k = k0; k < k1; k++) {
                     uint8_t* at = sm + s * stage_bytes;
-                    if (f >= ahead) {
-                        ok = mbar_wait(&empty[s], (f / g.stages - 1) & 1, failed);
+                    if (issued >= ahead) {
+                        ok = mbar_wait(&empty[s], phase, failed);
                         if (!ok) break;
                         mbar_expect(&full[s], stage_bytes);
-                        tma_load(at, &mw, k * KB, tile % nt * TM, &full[s]);
+                        tma_load(at, &mw, k * KB, y, &full[s]);
                     }
-                    tma_load(at + TM * KB, &mx, k * KB, tile / nt * g.tn, &full[s]);
-                    issued = f + 1;
+                    tma_load(at + TM * KB, &mx, k * KB, my, &full[s]);
+                    issued++;
+                    if (++s == g.stages) s = 0, phase ^= 1;
                 }
+            }
             if (*failed || !ok)   // everything that is under way lands before the CTA ends
                 for (int i = max(0, issued - g.stages); i < issued; i++) mbar_drain(&full[i % g.stages], (i / g.stages) & 1);
         }
-    } else if (warp == 5) {
+    } else if (warp == EW + 1) {
         if (lane == 0) {
             // D int32, A and B signed, K-major, N = tn, M = 128
             const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(g.tn >> 3) << 17) | ((TM >> 4) << 24);
-            int f = 0, i = 0;
+            int f = 0, i = 0, s = 0;
+            uint32_t phase = 0;
+            const uint64_t da0 = sw128_desc(saddr(sm)), db0 = sw128_desc(saddr(sm + TM * KB));
             bool ok = true;
             for (int tile = first; tile < tiles && ok; tile += stride, i++) {
                 if (i >= 2) ok = mbar_wait(&acc_free[i & 1], ((i >> 1) - 1) & 1, failed);
                 const uint32_t d = tmem + (i & 1) * (cols / 2);
+                uint32_t add = 0;   // the tile's first product overwrites
                 for (int k = k0; k < k1 && ok; k++, f++) {
-                    const int s = f % g.stages;
-                    ok = mbar_wait(&full[s], (f / g.stages) & 1, failed);
+                    ok = mbar_wait(&full[s], phase, failed);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t da = sw128_desc(saddr(sm + s * stage_bytes));
-                    const uint64_t db = sw128_desc(saddr(sm + s * stage_bytes + TM * KB));
+                    const uint64_t at = (uint64_t)(uint32_t)(s * (stage_bytes >> 4));
+                    const uint64_t da = da0 + at, db = db0 + at;
 #pragma unroll
-                    for (int x = 0; x < KB / 32; x++)
+                    for (int x = 0; x < KB / 32; x++) {
                         asm volatile(
                             "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                             "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                            "l"(da + 2 * x), "l"(db + 2 * x), "r"(idesc), "r"((k > k0 || x) ? 1 : 0));
+                            "l"(da + 2 * x), "l"(db + 2 * x), "r"(idesc), "r"(add));
+                        add = 1;
+                    }
                     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                                      saddr(&empty[s]))
                                  : "memory");
+                    if (++s == g.stages) s = 0, phase ^= 1;
                 }
                 if (ok)
                     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
@@ -310,47 +322,51 @@ __global__ void __launch_bounds__(GT, 1)
         }
     } else {
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        T* out = reinterpret_cast<T*>(g.out);
-        const T* res = reinterpret_cast<const T*>(g.res);
+        const int quad = warp & 3, side = warp >> 2;
         int i = 0;
         for (int tile = first; tile < tiles; tile += stride, i++) {
-            const int m0 = tile / nt * g.tn, n = tile % nt * TM + 32 * warp + lane;
+            const int m0 = tile / nt * g.tn, n = tile % nt * TM + 32 * quad + lane;
             const bool n_ok = n < g.N;
             const float sw = n_ok ? g.sw[n] : 0.0f;
+            float* sa = s_sa[i & 1];   // the other one may still be read
+            if (tid < g.tn) sa[tid] = m0 + tid < g.M ? g.sa[m0 + tid] : 0.0f;
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * EW) : "memory");
             const bool ok = mbar_wait(&acc_full[i & 1], (i >> 1) & 1, failed);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t d = tmem + (i & 1) * (cols / 2) + ((uint32_t)(32 * warp) << 16);
+            const uint32_t d = tmem + (i & 1) * (cols / 2) + ((uint32_t)(32 * quad) << 16);
             if (g.splits > 1) {
                 // own sums to shared memory (its stages are no longer in use), [column][channel]
                 int* part = reinterpret_cast<int*>(sm);
-                for (int c = 0; c < g.tn && ok; c += 16) {
+                for (int c = 16 * side; c < g.tn && ok; c += 32) {
                     uint32_t v[16];
                     tmem_ld<16>(v, d + c);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                    for (int x = 0; x < 16; x++) part[(c + x) * TM + 32 * warp + lane] = (int)v[x];
+                    for (int x = 0; x < 16; x++) part[(c + x) * TM + 32 * quad + lane] = (int)v[x];
                 }
                 break;   // one tile per cluster
             }
-            for (int c = 0; c < g.tn && m0 + c < g.M; c += 16) {
+            T* out = reinterpret_cast<T*>(g.out) + (size_t)(m0 + 16 * side) * g.os + n;
+            const T* res = g.res ? reinterpret_cast<const T*>(g.res) + (size_t)(m0 + 16 * side) * g.rs + n : nullptr;
+            for (int c = 16 * side; c < g.tn && m0 + c < g.M; c += 32) {
                 uint32_t v[16];
                 tmem_ld<16>(v, d + c);
-                const int m = m0 + c + (lane & 15);
-                const float sal = m < g.M ? g.sa[m] : 0.0f;
-                float r[16];
-                if (res)
+                const int left = n_ok ? g.M - m0 - c : 0;   // columns with an output
+                float r[16], s[16];
 #pragma unroll
-                    for (int x = 0; x < 16; x++)
-                        r[x] = n_ok && m0 + c + x < g.M ? to_f32(res[(size_t)(m0 + c + x) * g.rs + n]) : 0.0f;
+                for (int x = 0; x < 16; x++) r[x] = res && x < left ? to_f32(res[x * g.rs]) : 0.0f;
+#pragma unroll
+                for (int x = 0; x < 16; x += 4) *reinterpret_cast<float4*>(&s[x]) = *reinterpret_cast<const float4*>(sa + c + x);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                 for (int x = 0; x < 16; x++) {
-                    const float sa = __shfl_sync(0xffffffffu, sal, x);
-                    float o = (float)(int)v[x] * (sa * sw);
+                    float o = (float)(int)v[x] * (s[x] * sw);
                     if (res) o += r[x];
                     if (!ok) o = __int_as_float(0x7fc00000);
-                    if (n_ok && m0 + c + x < g.M) from_f32(o, out[(size_t)(m0 + c + x) * g.os + n]);
+                    if (x < left) from_f32(o, out[x * g.os]);
                 }
+                out += 32 * g.os;
+                if (res) res += 32 * g.rs;
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             mbar_arrive(&acc_free[i & 1]);
@@ -360,32 +376,42 @@ __global__ void __launch_bounds__(GT, 1)
     if (g.splits > 1) {   // every CTA's sums are in shared memory
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (warp < 4 && first < tiles) {
-            T* out = reinterpret_cast<T*>(g.out);
-            const T* res = reinterpret_cast<const T*>(g.res);
-            const int m0 = first / nt * g.tn, n = first % nt * TM + 32 * warp + lane;
+        if (warp < EW && first < tiles) {
+            const int m0 = first / nt * g.tn, quad = warp & 3, row = 32 * quad + lane, n = first % nt * TM + row;
             const float sw = n < g.N ? g.sw[n] : 0.0f;
-            bool bad = false;
-            for (int r = 0; r < g.splits; r++) {
-                uint32_t at, v;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(saddr(&s_failed)), "r"(r));
-                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-                bad |= v != 0;
+            uint32_t peer[MAX_SPLITS], bad = 0;
+#pragma unroll
+            for (int r = 0; r < MAX_SPLITS; r++) {
+                const int p = r < g.splits ? r : 0;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer[r]) : "r"(saddr(sm) + row * 4), "r"(p));
             }
-            for (int c = rank; c < g.tn && m0 + c < g.M; c += g.splits) {
-                int acc = 0;
-                const uint32_t mine = saddr(sm) + (uint32_t)(c * TM + 32 * warp + lane) * 4;
-                for (int r = 0; r < g.splits; r++) {
-                    uint32_t at, v;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine), "r"(r));
-                    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-                    acc += (int)v;
+            {
+                uint32_t at;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(saddr(&s_failed)), "r"(lane % g.splits));
+                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(bad) : "r"(at) : "memory");
+                bad = __any_sync(0xffffffffu, bad != 0);
+            }
+            T* out = reinterpret_cast<T*>(g.out) + (size_t)m0 * g.os + n;
+            const T* res = g.res ? reinterpret_cast<const T*>(g.res) + (size_t)m0 * g.rs + n : nullptr;
+            const int end = min(g.tn, g.M - m0);
+#pragma unroll 2
+            for (int c = rank + g.splits * (warp >> 2); c < end; c += 2 * g.splits) {
+                uint32_t v[MAX_SPLITS];
+#pragma unroll
+                for (int r = 0; r < MAX_SPLITS; r++) {
+                    v[r] = 0;
+                    if (r < g.splits)
+                        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v[r]) : "r"(peer[r] + c * TM * 4) : "memory");
                 }
+                const float q = res && n < g.N ? to_f32(res[(size_t)c * g.rs]) : 0.0f;
+                int acc = 0;
+#pragma unroll
+                for (int r = 0; r < MAX_SPLITS; r++) acc += (int)v[r];
                 if (n < g.N) {
-                    float o = (float)acc * (g.sa[m0 + c] * sw);
-                    if (res) o += to_f32(res[(size_t)(m0 + c) * g.rs + n]);
+                    float o = (float)acc * (s_sa[0][c] * sw);
+                    if (res) o += q;
                     if (bad) o = __int_as_float(0x7fc00000);
-                    from_f32(o, out[(size_t)(m0 + c) * g.os + n]);
+                    from_f32(o, out[(size_t)c * g.os]);
                 }
             }
         }
@@ -395,11 +421,11 @@ __global__ void __launch_bounds__(GT, 1)
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
+    if (warp == EW + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
 }
 
 // ---------------------------------------------------------------- its launch
-constexpr int SMEM_MAX = 227 * 1024 - 2048;   // beside the barriers
+constexpr int SMEM_MAX = 227 * 1024 - 4096;   // beside the barriers and the scales
 
 struct MatPlan {
     int tn, splits, stages, ctas;
@@ -417,7 +443,7 @@ MatPlan plan_mat(int M, int N, int kp, int sms) {
         if (tn > 16 && tn - 16 >= M) break;   // wider than the tokens
         const long long tiles = (long long)nt * ((M + tn - 1) / tn);
         const double step = fmax(fmax(2.0 * tn, 128.0), (TM * KB + tn * KB) / 32.0);
-        for (int s = 1; s <= 8 && s <= kt; s++) {
+        for (int s = 1; s <= MAX_SPLITS && s <= kt; s++) {
             if (s > 1 && (tiles * s > sms || tn * TM * 4 > SMEM_MAX - 1024)) break;
             const long long waves = (tiles * s + sms - 1) / sms;
             const double cost = (double)waves * ((kt + s - 1) / s) * step + 8.0 * tn + (s > 1 ? 1500.0 + 4.0 * tn : 0.0);
