@@ -16,7 +16,8 @@ def randn(seed, *shape):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 2048), (3, 31), (7, 155), (300, 128), (2, 9001), (1, 131072), (129, 768)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 2048), (3, 31), (7, 155), (300, 128), (2, 9001), (1, 131072), (129, 768), (2100, 400),
+                                       (2050, 4100), (2048, 33)])
 @pytest.mark.parametrize("norm", [False, True])
 def test_rows(rows, cols, dtype, norm):
     from tinygiant_b200.int8 import quantize_rows

@@ -18,8 +18,6 @@ namespace tg {
 
 namespace {
 
-constexpr int QT = 256;   // threads of the row quantiser
-
 struct QuantArgs {
     const void* x;
     long long xs;
@@ -30,76 +28,177 @@ struct QuantArgs {
     float* scales;
 };
 
-// rint(127 y / top) for y = x (or x * w, unrounded), |y| <= top, in exact arithmetic: the
-// fp32 quotient is off by less than 2^-15, so only values that close to a border need the
-// 64-bit one (127 x is exact there; x * w * 127 and the quotient round at 2^-53).
-__device__ __forceinline__ int i8_code(float x, float w, double top, float inv) {
-    const float r = x * w * inv;
-    const float c = rintf(r);
-    if (fabsf(fabsf(r - c) - 0.5f) > 1e-3f) return (int)c;
-    return (int)rint((double)x * w * 127.0 / top);
+// 16 bytes of x as floats, and their norm weights: in one piece (ALL), or element by element
+// with zeros behind the row.
+template <bool ALL, int V, typename T>
+__device__ __forceinline__ void load_piece(float (&v)[V], const T* x, int at, int cols) {
+    if constexpr (ALL) {
+        const uint4 u = *reinterpret_cast<const uint4*>(x + at);
+        const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = to_f32(t[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = at + i < cols ? to_f32(x[at + i]) : 0.0f;
+    }
+}
+template <bool NORM, bool ALL, int V>
+__device__ __forceinline__ void load_norm(float (&w)[V], const float* norm, int at, int cols) {
+    if constexpr (NORM && ALL) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(&w[i]) = *reinterpret_cast<const float4*>(norm + at + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) w[i] = NORM ? (at + i < cols ? norm[at + i] : 0.0f) : 1.0f;
+    }
 }
 
-template <int DT, bool NORM>
-__global__ void __launch_bounds__(QT) k_i8_rows(QuantArgs a) {
-    using T = typename Elem<DT>::T;
-    __shared__ double s_top[QT / 32];
-    __shared__ float s_ss[QT / 32];
-    __shared__ int s_bad;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the product's weights may come
-    const int row = blockIdx.x, tid = threadIdx.x;
-    const T* x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.xs;
-    double top = 0.0;
-    float ss = 0.0f;
-    bool bad = false;
-    if (tid == 0) s_bad = 0;
-    __syncthreads();
-    for (int i = tid; i < a.cols; i += QT) {
-        const float v = to_f32(x[i]);
-        bad |= !(fabsf(v) <= 3.4028235e38f);
-        double y = v;
-        if (NORM) {
-            const float w = a.norm[i];
-            bad |= !(fabsf(w) <= 3.4028235e38f);
-            y *= w;
-            ss += v * v;
-        }
-        top = fmax(top, fabs(y));
+__device__ __forceinline__ float max_nan(float x, float y) {   // NaN if either is
+    float z;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+    return z;
+}
+
+// rint(127 x w / top) in 64 bits: 127 x is exact, x w and the quotient round at 2^-53.
+__device__ __noinline__ int i8_code_exact(float x, float w, double top) { return (int)rint((double)x * w * 127.0 / top); }
+
+// The codes of a piece, packed: rint(127 y / top) for y = x (or x * w, unrounded), |y| <= top, in
+// exact arithmetic.  Adding 1.5 * 2^23 rounds the fp32 quotient to a whole number, ties to even,
+// and leaves it in the low byte.  That quotient is off by less than 2^-15, so only what comes
+// that close to a border (2 in 10000, for a margin of 1e-4) needs the 64-bit one.
+template <int V>
+__device__ __forceinline__ void i8_codes(uint32_t (&c)[V / 4], const float (&x)[V], const float (&w)[V], double top, float inv) {
+    float t[V], far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const float r = x[i] * (w[i] * inv);
+        t[i] = __fadd_rn(r, 12582912.0f);
+        far = fmaxf(far, fabsf(r - __fsub_rn(t[i], 12582912.0f)));
     }
+    if (far >= 0.4999f) {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (fabsf(x[i] * (w[i] * inv) - __fsub_rn(t[i], 12582912.0f)) >= 0.4999f)
+                t[i] = __int_as_float(i8_code_exact(x[i], w[i], top));
+    }
+#pragma unroll
+    for (int i = 0; i < V; i += 4)
+        c[i / 4] = __byte_perm(__byte_perm(__float_as_uint(t[i]), __float_as_uint(t[i + 1]), 0x0040),
+                               __byte_perm(__float_as_uint(t[i + 2]), __float_as_uint(t[i + 3]), 0x0040), 0x5410);
+}
+
+// G warps per row, two passes: the largest |y| and the sum of squares, then the codes.  The
+// largest y = x * w has to be exact: its fp32 rounding is found first, then what the rounding
+// lost, in the pieces that hold it.  The second pass reads the row again, from L1: rolled loops
+// over it beat rows held in registers, whose unrolled code did not fit the instruction cache
+// (8100 x 2048 bf16 behind a norm: 41 to 56 us).
+//
+// Bound by the instructions, about 15 an element, for many rows: a warp each and no barrier
+// (G = 1).  For few rows, by latency: a CTA each (G = 8).
+template <int DT, bool NORM, bool VEC, int G>
+__global__ void __launch_bounds__(256) k_i8_rows(QuantArgs a) {
+    using T = typename Elem<DT>::T;
+    constexpr int V = 16 / sizeof(T), NT = 32 * G;
+    static_assert(G == 1 || G == 8, "a warp or a CTA of 256 threads per row");
+    __shared__ float s_hi[8], s_ss[8];
+    __shared__ double s_top[8];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the product's weights may come
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const int row = G == 1 ? blockIdx.x * 8 + wid : blockIdx.x, tid = G == 1 ? lane : threadIdx.x;
+    if (row >= a.rows) return;
+    const T* x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.xs;
+    const int pieces = a.kp / V;
+    const int whole = VEC ? a.cols / V : 0;   // pieces that load in one go
+    float hi = 0.0f, ss = 0.0f;               // hi: NaN once a value is
+    uint32_t where = 0;                       // the thread's pieces whose largest is hi; bit 31: those from 31 on
+    // f(values, weights, first column, its number) of every piece of the row that the thread owns
+    auto each = [&](auto&& f) {
+        float v[V], w[V];
+        int i = 0, c = tid;
+#pragma unroll 2
+        for (; c < whole; c += NT, i++) {
+            load_piece<true>(v, x, c * V, a.cols);
+            load_norm<NORM, true>(w, a.norm, c * V, a.cols);
+            f(v, w, c * V, min(i, 31));
+        }
+#pragma unroll 1
+        for (; c < pieces; c += NT, i++) {
+            load_piece<false>(v, x, c * V, a.cols);
+            load_norm<NORM, false>(w, a.norm, c * V, a.cols);
+            f(v, w, c * V, min(i, 31));
+        }
+    };
+    each([&](const float (&v)[V], const float (&w)[V], int, int at) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            top = max_nan(top, fabsf(NORM ? __fmul_rn(v[i], w[i]) : v[i]));
+            if (NORM) ss = fmaf(v[i], v[i], ss);
+        }
+        where = top > hi ? 1u << at : top == hi ? where | 1u << at : where;
+        hi = max_nan(hi, top);
+    });
+    const float own = hi;
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
-        top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        if (NORM) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     }
-    if (bad) s_bad = 1;
-    if ((tid & 31) == 0) {
-        s_top[tid >> 5] = top;
-        s_ss[tid >> 5] = ss;
-    }
-    __syncthreads();
-    ss = 0.0f;
+    if constexpr (G > 1) {
+        if (lane == 0) s_hi[wid] = hi, s_ss[wid] = ss;
+        __syncthreads();
+        ss = 0.0f;
 #pragma unroll
-    for (int i = 0; i < QT / 32; i++) {
-        top = fmax(top, s_top[i]);
-        ss += s_ss[i];
-    }
-    bad = s_bad || !(top <= 3.4028234663852886e38);
-    const float topf = __double2float_rn(top), inv = __fdiv_rn(127.0f, topf);
-    int8_t* out = a.codes + (size_t)row * a.kp;
-    // 127 / top overflows for a top this small: quotients then come from 64 bits
-    const bool tiny = !(inv <= 3.4028235e38f);
-    for (int i = tid; i < a.kp; i += QT) {
-        int c = 0;
-        if (i < a.cols && !bad && top > 0.0) {
-            const float v = to_f32(x[i]), w = NORM ? a.norm[i] : 1.0f;
-            c = tiny ? (int)rint((double)v * w * 127.0 / top) : i8_code(v, w, top, inv);
+        for (int i = 0; i < G; i++) {
+            hi = max_nan(hi, s_hi[i]);
+            ss += s_ss[i];
         }
-        out[i] = (int8_t)c;
     }
+    const bool poor = !(hi <= 3.4028235e38f);
+    double top = hi;
+    bool exact = false;   // codes from 64-bit quotients throughout
+    if (NORM && hi > 0.0f && !poor) {
+        double y = 0.0;   // the largest in 64 bits, where it may be
+        exact = hi < 1e-30f;   // what such products lose is beyond fp32, too
+        if (own == hi || exact)
+            each([&](const float (&v)[V], const float (&w)[V], int, int at) {
+                if ((where >> at & 1) || exact)
+#pragma unroll
+                    for (int i = 0; i < V; i++)
+                        if (exact || fabsf(__fmul_rn(v[i], w[i])) == hi) y = fmax(y, fabs((double)v[i] * w[i]));
+            });
+        __syncwarp();
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) y = fmax(y, __shfl_xor_sync(0xffffffffu, y, o));
+        if constexpr (G > 1) {
+            if (lane == 0) s_top[wid] = y;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < G; i++) y = fmax(y, s_top[i]);
+        }
+        top = y;
+    }
+    const float topf = __double2float_rn(top), inv = __fdiv_rn(127.0f, topf);
+    const bool none = poor || !(topf <= 3.4028235e38f) || top == 0.0;
+    exact |= !(inv <= 3.4028235e38f);   // 127 / top overflows for a top this small
+    int8_t* out = a.codes + (size_t)row * a.kp;
+    each([&](const float (&v)[V], const float (&w)[V], int at, int) {
+        uint32_t c[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; i++) c[i] = 0;
+        if (!none && !exact) i8_codes(c, v, w, top, inv);
+        if (!none && exact)
+#pragma unroll
+            for (int i = 0; i < V; i++) c[i / 4] |= (uint32_t)(i8_code_exact(v[i], w[i], top) & 255) << (8 * (i % 4));
+        if constexpr (V == 8)
+            *reinterpret_cast<uint2*>(out + at) = make_uint2(c[0], c[1]);
+        else
+            *reinterpret_cast<uint32_t*>(out + at) = c[0];
+    });
     if (tid == 0) {
         float s = __fdiv_rn(topf, 127.0f);
         if (NORM) s *= __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.cols), a.eps)));
-        a.scales[row] = bad ? __int_as_float(0x7fc00000) : s;
+        a.scales[row] = poor || !(topf <= 3.4028235e38f) ? __int_as_float(0x7fc00000) : s;
     }
 }
 
@@ -526,10 +625,21 @@ cudaError_t launch_mat(MatArgs g, const int8_t* x, const int8_t* w, int kp, cuda
 
 template <int DT>
 cudaError_t launch_rows(const QuantArgs& a, cudaStream_t s) {
-    if (a.norm)
-        k_i8_rows<DT, true><<<a.rows, QT, 0, s>>>(a);
-    else
-        k_i8_rows<DT, false><<<a.rows, QT, 0, s>>>(a);
+    constexpr int E = DT == TGX_F32 ? 4 : 2;
+    const bool vec = ((uintptr_t)a.x | (uintptr_t)(a.xs * E) | (uintptr_t)a.norm) % 16 == 0;
+    // a warp per row once that fills the device (148 SMs of 24 such warps) and rows are no longer
+    // than a few thousand: 8100 x 2048 bf16 took 41 us a CTA each
+    if (a.rows >= 2048 && a.kp <= 8192) {
+        const int grid = (a.rows + 7) / 8;
+        if (a.norm)
+            vec ? k_i8_rows<DT, true, true, 1><<<grid, 256, 0, s>>>(a) : k_i8_rows<DT, true, false, 1><<<grid, 256, 0, s>>>(a);
+        else
+            vec ? k_i8_rows<DT, false, true, 1><<<grid, 256, 0, s>>>(a) : k_i8_rows<DT, false, false, 1><<<grid, 256, 0, s>>>(a);
+    } else if (a.norm) {
+        vec ? k_i8_rows<DT, true, true, 8><<<a.rows, 256, 0, s>>>(a) : k_i8_rows<DT, true, false, 8><<<a.rows, 256, 0, s>>>(a);
+    } else {
+        vec ? k_i8_rows<DT, false, true, 8><<<a.rows, 256, 0, s>>>(a) : k_i8_rows<DT, false, false, 8><<<a.rows, 256, 0, s>>>(a);
+    }
     return cudaGetLastError();
 }
 
