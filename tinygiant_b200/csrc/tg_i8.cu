@@ -446,26 +446,46 @@ __global__ void __launch_bounds__(GT, 1)
                 break;   // one tile per cluster
             }
             T* out = reinterpret_cast<T*>(g.out) + (size_t)(m0 + 16 * side) * g.os + n;
-            const T* res = g.res ? reinterpret_cast<const T*>(g.res) + (size_t)(m0 + 16 * side) * g.rs + n : nullptr;
-            for (int c = 16 * side; c < g.tn && m0 + c < g.M; c += 32) {
-                uint32_t v[16];
-                tmem_ld<16>(v, d + c);
-                const int left = n_ok ? g.M - m0 - c : 0;   // columns with an output
-                float r[16], s[16];
+            if (!g.res && ok && m0 + g.tn <= g.M && tile % nt * TM + TM <= g.N) {   // nothing to ask per output
+                for (int c = 16 * side; c < g.tn; c += 32) {
+                    uint32_t v[16];
+                    tmem_ld<16>(v, d + c);
+                    float s[16];
 #pragma unroll
-                for (int x = 0; x < 16; x++) r[x] = res && x < left ? to_f32(res[x * g.rs]) : 0.0f;
+                    for (int x = 0; x < 16; x += 4) *reinterpret_cast<float4*>(&s[x]) = *reinterpret_cast<const float4*>(sa + c + x);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    T* to = out;
 #pragma unroll
-                for (int x = 0; x < 16; x += 4) *reinterpret_cast<float4*>(&s[x]) = *reinterpret_cast<const float4*>(sa + c + x);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    float o = (float)(int)v[x] * (s[x] * sw);
-                    if (res) o += r[x];
-                    if (!ok) o = __int_as_float(0x7fc00000);
-                    if (x < left) from_f32(o, out[x * g.os]);
+                    for (int x = 0; x < 16; x++) {
+                        from_f32((float)(int)v[x] * (s[x] * sw), *to);
+                        to += g.os;
+                    }
+                    out += 32 * g.os;
                 }
-                out += 32 * g.os;
-                if (res) res += 32 * g.rs;
+            } else {
+                const T* res = g.res ? reinterpret_cast<const T*>(g.res) + (size_t)(m0 + 16 * side) * g.rs + n : nullptr;
+                for (int c = 16 * side; c < g.tn && m0 + c < g.M; c += 32) {
+                    uint32_t v[16];
+                    tmem_ld<16>(v, d + c);
+                    const int left = n_ok ? g.M - m0 - c : 0;   // columns with an output
+                    float r[16], s[16];
+#pragma unroll
+                    for (int x = 0; x < 16; x++) r[x] = res && x < left ? to_f32(res[x * g.rs]) : 0.0f;
+#pragma unroll
+                    for (int x = 0; x < 16; x += 4) *reinterpret_cast<float4*>(&s[x]) = *reinterpret_cast<const float4*>(sa + c + x);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    T* to = out;
+#pragma unroll
+                    for (int x = 0; x < 16; x++) {
+                        float o = (float)(int)v[x] * (s[x] * sw);
+                        if (res) o += r[x];
+                        if (!ok) o = __int_as_float(0x7fc00000);
+                        if (x < left) from_f32(o, *to);
+                        to += g.os;
+                    }
+                    out += 32 * g.os;
+                    if (res) res += 32 * g.rs;
+                }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             mbar_arrive(&acc_free[i & 1]);
