@@ -86,8 +86,9 @@ __device__ __forceinline__ KvqPlace kvq_place(const KvqBatch& b, const KvqCache&
         if (lane == 0) kvq_flag(b, TGX_KVQ_BAD_LENGTH);
         return p;
     }
-    p.page = b.table[(size_t)p.seq * b.max_pages + (int)(row / c.pt)];
-    p.tok = (int)(row % c.pt);
+    const int r = (int)row, at = r / c.pt;   // max_pages * pt fits 32 bits
+    p.page = b.table[(size_t)p.seq * b.max_pages + at];
+    p.tok = r - at * c.pt;
     if (p.page < 0 || p.page >= c.n_pages) {
         if (lane == 0) kvq_flag(b, TGX_KVQ_BAD_PAGE);
         return p;
