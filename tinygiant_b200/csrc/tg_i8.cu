@@ -12,6 +12,7 @@
 
 #include <cmath>
 
+#include "tg_mbar.cuh"
 #include "tg_serve.cuh"
 
 namespace tg {
@@ -239,72 +240,12 @@ constexpr int MAX_STAGES = 12;
 constexpr int MAX_SPLITS = 4;     // larger clusters of one CTA per SM wait for room in a GPC: 8 took 20 us where 4 take 15
 constexpr int EW = 8;             // epilogue warps
 constexpr int GT = 32 * (EW + 2); // threads
-constexpr long long WAIT_CYCLES = 2000000000ll;   // about a second
-
-__device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint64_t* m, int n) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(saddr(m)), "r"(n));
-}
-__device__ __forceinline__ void mbar_expect(uint64_t* m, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(saddr(m)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* m) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(saddr(m)) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint64_t* m, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(saddr(m)), "r"(parity)
-        : "memory");
-    return done;
-}
-// Waits for the phase; false once the limit is over here or a wait has failed elsewhere in the CTA.
-__device__ __forceinline__ bool mbar_wait(uint64_t* m, uint32_t parity, volatile int* failed) {
-    if (mbar_try(m, parity)) return true;
-    const long long t0 = clock64();
-    while (!mbar_try(m, parity)) {
-        if (*failed) return false;
-        if (clock64() - t0 > WAIT_CYCLES) {
-            *failed = 1;
-            return false;
-        }
-    }
-    return true;
-}
-// The same for what must land before the CTA may end.
-__device__ __forceinline__ void mbar_drain(uint64_t* m, uint32_t parity) {
-    const long long t0 = clock64();
-    while (!mbar_try(m, parity) && clock64() - t0 < WAIT_CYCLES) {
-    }
-}
-
 __device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, uint64_t* mbar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
             saddr(dst)),
         "l"(map), "r"(x), "r"(y), "r"(saddr(mbar))
         : "memory");
-}
-
-// K-major operand in 128-byte swizzle: rows of 128 bytes, 8-row atoms 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr) {
-    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
-           (uint64_t)2 << 61;
-}
-
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t (&v)[N], uint32_t at);
-template <>
-__device__ __forceinline__ void tmem_ld<16>(uint32_t (&v)[16], uint32_t at) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-        "[%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(at));
 }
 
 template <int DT>

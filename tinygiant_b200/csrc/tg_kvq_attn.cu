@@ -39,7 +39,7 @@
 #include <cmath>
 #include <mutex>
 
-#include "tg_serve.cuh"
+#include "tg_kvq_attn.cuh"
 
 namespace tg {
 
@@ -49,21 +49,6 @@ constexpr int DEEP_WARPS = 4;         // warps of a worker that share an item
 constexpr float P_EXP = 6.0f;        // p is held times 2^P_EXP
 constexpr float P_SLACK = 4.0f;      // and may exceed that by 2^P_SLACK before m moves
 constexpr int V_LOW = 2, V_HIGH = 5; // V scales are held in 2^V_LOW .. 2^V_HIGH at the largest: 2^(6 + 4 + 5) < 65504
-
-struct AttnKvqArgs {
-    KvqCache c;
-    KvqBatch b;
-    int T, NH, R;       // R = NH / nkv
-    const void* q;
-    long long qs;
-    void* out;
-    long long os;
-    float scale;        // times log2(e)
-    uint32_t k1024;     // fp16 1024 twice
-    int workers;
-    float* slots;       // [workers][2] partial results: m, l [rows], O [rows][HD]
-    int* heads;         // [workers][2][4] what a slot holds: kind, token row base, kv head, query rows
-};
 
 // What beginning an item costs beside its granules, in a warp's granules: about 5 us measured
 // (queries, first copies, joining the warps), against 0.6 us for a granule.
@@ -75,8 +60,6 @@ constexpr int workers_per_sm(int warps) { return warps > 1 ? 4 : 12; }
 constexpr int MAX_WORKERS = MAX_SMS * workers_per_sm(1);
 
 enum { SLOT_NONE = 0, SLOT_MORE = 1, SLOT_LAST = 2 };
-
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -97,95 +80,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // an 8 x 8 tile 
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ __half2 as_h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
-__device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
-
-// Two codes of the lower (bits 0 .. 3 of each halfword) or the upper nibbles (4 .. 7) as
-// fp16: code - 8, or, RAW, code * 2^-24 and code * 2^-20.
-// `k1024` is 1024 twice, in a register: one three-input operation then masks and merges.
-template <bool RAW>
-__device__ __forceinline__ uint32_t codes_lo(uint32_t x, uint32_t k1024) {
-    if constexpr (RAW) return x & 0x000f000fu;
-    uint32_t y;
-    asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(y) : "r"(x), "r"(k1024));
-    return as_u32(__hadd2(as_h2(y), __float2half2_rn(-1032.0f)));
-}
-template <bool RAW>
-__device__ __forceinline__ uint32_t codes_hi(uint32_t x, uint32_t k1024) {
-    if constexpr (RAW) return x & 0x00f000f0u;
-    uint32_t y;
-    asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xEA;" : "=r"(y) : "r"(x), "r"(k1024));
-    return as_u32(__hfma2(as_h2(y), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f)));
-}
-
-constexpr uint32_t NO_GRANULE = 0xffffffffu;
-
-// N words, in the widest loads that their alignment allows.
-template <int N>
-__device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
-    if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) *reinterpret_cast<uint4*>(&w[i]) = *reinterpret_cast<const uint4*>(p + 4 * i);
-    } else if constexpr (N % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 2) *reinterpret_cast<uint2*>(&w[i]) = *reinterpret_cast<const uint2*>(p + 4 * i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) w[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
-    }
-}
-// N fp16 scales as floats.
-template <int N>
-__device__ __forceinline__ void load_scales(float (&d)[N], const uint8_t* p) {
-    if constexpr (N % 2 == 0) {
-        uint32_t w[N / 2];
-        load_words<N / 2>(w, p);
-#pragma unroll
-        for (int i = 0; i < N; i++) d[i] = i & 1 ? __high2float(as_h2(w[i / 2])) : __low2float(as_h2(w[i / 2]));
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) d[i] = __half2float(*reinterpret_cast<const __half*>(p + 2 * i));
-    }
-}
-__device__ __forceinline__ float2 load2(const float* p) { return *reinterpret_cast<const float2*>(p); }
-__device__ __forceinline__ float2 load2(const __nv_bfloat16* p) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
-}
-__device__ __forceinline__ float2 load2(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
-
-// A sequence's share of the call.
-struct SeqInfo {
-    int s0, n;          // first new token, how many are attended for
-    long long len;      // cached rows within the table
-    int off;            // new token i sees the rows below off + i + 1 (may be negative)
-    int tiles, grans;   // row tiles per kv head; units per tile (at least one)
-};
-
-__device__ __forceinline__ long long quotient(long long x, long long y) {
-    if ((x | y) < 0x100000000ll) return (uint32_t)x / (uint32_t)y;
-    return x / y;
-}
-
-__device__ __forceinline__ SeqInfo seq_info(const AttnKvqArgs& a, int b, int tile_rows) {
-    SeqInfo s;
-    const int s0 = a.b.q_start[b], s1 = a.b.q_start[b + 1];
-    s.s0 = s0;
-    s.n = s0 >= 0 && s1 > s0 && s1 <= a.T ? s1 - s0 : 0;
-    const long long cap = (long long)a.b.max_pages * a.c.pt, len = a.b.kv_lens[b];
-    const long long off = len - s.n;
-    s.off = (int)(off < -(1ll << 30) ? -(1ll << 30) : off);
-    s.len = len < 0 ? 0 : len > cap ? cap : len;
-    s.n = min(s.n, a.b.max_new);
-    s.tiles = (int)(((long long)s.n * a.R + tile_rows - 1) / tile_rows);
-    s.grans = max(1, (int)((s.len + 15) >> 4));
-    return s;
-}
-
 // Four CTAs of four warps per SM (128 registers a thread) where that leaves nothing to spill.
 constexpr int min_ctas(int nb, int nt) { return nb <= 3 && nt == 1 ? 4 : nb * nt <= 4 ? 3 : 2; }
 
@@ -1045,7 +939,15 @@ cudaError_t launch_attn_nb(AttnKvqArgs a, void* scratch, size_t scratch_bytes, c
 template <int DT>
 cudaError_t launch_t(const AttnKvqArgs& a, void* scratch, size_t n, cudaStream_t s) { TG_NB(DT, launch_attn_nb, a, scratch, n, s) }
 
-cudaError_t launch_attn(int dtype, const AttnKvqArgs& a, void* scratch, size_t n, cudaStream_t s) {
+cudaError_t launch_attn(int dtype, AttnKvqArgs a, void* scratch, size_t n, cudaStream_t s) {
+    if (attn_tc_takes(dtype, a.c, a.b, a.R)) {
+        const size_t tc = attn_tc_scratch(a.c, a.b);
+        if (n < tc) return cudaErrorInvalidValue;
+        cudaError_t e = launch_attn_tc(dtype, a, scratch, &a.only, s);
+        if (e != cudaSuccess) return e;
+        scratch = (uint8_t*)scratch + tc;
+        n -= tc;
+    }
     return dtype == TGX_F32    ? launch_t<TGX_F32>(a, scratch, n, s)
            : dtype == TGX_BF16 ? launch_t<TGX_BF16>(a, scratch, n, s)
                                : launch_t<TGX_F16>(a, scratch, n, s);
@@ -1067,7 +969,7 @@ extern "C" size_t tgx_kvq_attention_scratch_bytes(const tgx_kvq_cache* cache, co
     for (int two = 0; two < 2; two++)
         most = std::max(most, tg::attn_scratch(tg::shape_of(c, b, n_heads / c.nkv, two, tg::MAX_SMS * tg::workers_per_sm(1),
                                                             tg::MAX_SMS * tg::workers_per_sm(tg::DEEP_WARPS)), c.hd));
-    return most;
+    return most + tg::attn_tc_scratch(c, b);
 }
 
 extern "C" int tgx_kvq_attention(const tgx_kvq_cache* cache, const tgx_kvq_batch* batch, int dtype, int n_tokens,
@@ -1094,7 +996,7 @@ extern "C" int tgx_kvq_attention(const tgx_kvq_cache* cache, const tgx_kvq_batch
     if (dev.rc != TG_OK || n_tokens == 0) return dev.rc;
     const float sc = (scale > 0.0f ? scale : 1.0f / sqrtf((float)cache->head_dim)) * 1.44269504088896340736f;
     tg::AttnKvqArgs a{tg::kvq_cache(*cache), tg::kvq_batch(*batch), n_tokens, n_heads, n_heads / cache->n_kv_heads, q,
-                      q_stride, out, out_stride, sc, 0x64006400u, 0, nullptr, nullptr};
+                      q_stride, out, out_stride, sc, 0x64006400u, 0, nullptr, nullptr, nullptr};
     cudaError_t e = tg::launch_attn(dtype, a, scratch, scratch_bytes, (cudaStream_t)stream);
     return e == cudaSuccess ? TG_OK : tg::serve_fail(TG_ECUDA, fn, cudaGetErrorString(e));
 }
