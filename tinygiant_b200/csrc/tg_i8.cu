@@ -322,37 +322,40 @@ __global__ void __launch_bounds__(GT, 1)
                 for (int i = max(0, issued - g.stages); i < issued; i++) mbar_drain(&full[i % g.stages], (i / g.stages) & 1);
         }
     } else if (warp == EW + 1) {
-        if (lane == 0) {
+        {
             // D int32, A and B signed, K-major, N = tn, M = 128
             const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(g.tn >> 3) << 17) | ((TM >> 4) << 24);
             int f = 0, i = 0, s = 0;
             uint32_t phase = 0;
             const uint64_t da0 = sw128_desc(saddr(sm)), db0 = sw128_desc(saddr(sm + TM * KB));
-            bool ok = true;
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            bool ok = true;   // the warp is in step throughout; one lane issues
             for (int tile = first; tile < tiles && ok; tile += stride, i++) {
-                if (i >= 2) ok = mbar_wait(&acc_free[i & 1], ((i >> 1) - 1) & 1, failed);
-                const uint32_t d = tmem + (i & 1) * (cols / 2);
+                if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&acc_free[i & 1], ((i >> 1) - 1) & 1, failed));
+                const uint32_t d = tm + (i & 1) * (cols / 2);
                 uint32_t add = 0;   // the tile's first product overwrites
                 for (int k = k0; k < k1 && ok; k++, f++) {
-                    ok = mbar_wait(&full[s], phase, failed);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase, failed));
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t at = (uint64_t)(uint32_t)(s * (stage_bytes >> 4));
                     const uint64_t da = da0 + at, db = db0 + at;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int x = 0; x < KB / 32; x++) {
-                        asm volatile(
-                            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                            "l"(da + 2 * x), "l"(db + 2 * x), "r"(idesc), "r"(add));
-                        add = 1;
+                        for (int x = 0; x < KB / 32; x++)
+                            asm volatile(
+                                "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                                "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                                "l"(da + 2 * x), "l"(db + 2 * x), "r"(idesc), "r"(x ? 1u : add));
+                        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                                         saddr(&empty[s]))
+                                     : "memory");
                     }
-                    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                                     saddr(&empty[s]))
-                                 : "memory");
+                    __syncwarp();
+                    add = 1;
                     if (++s == g.stages) s = 0, phase ^= 1;
                 }
-                if (ok)
+                if (ok && elect_one())
                     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                                      saddr(&acc_full[i & 1]))
                                  : "memory");

@@ -2,25 +2,24 @@
 // tcgen05, for 16-bit types and heads of 64 or 128.
 //
 // A CTA has 256 query rows (new tokens x heads of one kv head) as two tiles of 128, and walks
-// the rows they see in tiles of 128 tokens:
-//   S = Q K^T     kind::f16, 128 x 128 fp32 in TMEM
+// the rows they see in tiles of 64 tokens:
+//   S = Q K^T     kind::f16, 128 x 64 fp32 in TMEM, two of them per query tile
 //   p = 2^(s - m) a thread per query row, reading its TMEM lane; P goes back over S as fp16
 //   O += P V      A from TMEM, B the transposed V tile
 // Codes are turned into fp16 values once per CTA and tile, code * d rounded to 11 bits, by four
 // warps that read the granules straight into registers (the next tile's while this one's are
-// converted) and write the 128-byte-swizzled operands; a ring of three slots holds K, V, K, ...
+// converted) and write the 128-byte-swizzled operands; a ring of six slots holds K, V, K, ...
 // The layout of the cache makes both K-major operands of 4-byte pieces that 32 lanes store
 // without a bank conflict: two dimensions of a token for K, two tokens of a dimension for V.
-// Two query tiles take turns: while one's softmax runs the tensor cores work on the other.
+// The scores of a tile are issued before the softmax of the one in front is waited for, so the
+// softmax warps go from tile to tile (with one S per query tile and tiles of 128 tokens they
+// waited: 254 us instead of TCUS for three prompts of up to 1500 tokens behind up to 2500).
 //
 // m moves, and O in TMEM is rescaled, only when a row's scores leave 2^SLACK of it.  q rows, K
 // and V are held in fp16 times powers of two: q's largest in 2^13 .. 2^14, the largest scale of
 // the sequence's head in 2^7 .. 2^8 (found by k_kvq_scan in front, which also marks sequences
 // with a scale that is not finite: a NaN behind a row's limit must not meet a probability of 0,
 // so those are left to tg_kvq_attn.cu's kernel).
-//
-// Bound by its three units about equally: a tile of 256 x 128 x 128 takes the tensor cores 2200
-// cycles, the 2^x units 2000, and the issue slots about 2300.
 //
 // Every wait is bounded; where one expires the CTA's outputs become NaN.
 #include "tg_kvq_attn.cuh"
@@ -31,8 +30,8 @@ namespace tg {
 namespace {
 
 constexpr int QT = 128;          // query rows of a tile
-constexpr int TK = 128;          // tokens of a tile
-constexpr int SLOTS = 3;
+constexpr int TK = 64;           // tokens of a tile: a granule per conversion warp
+constexpr int SLOTS = 6;
 constexpr int SW = 8, DW = 4;    // softmax and conversion warps; one more for the MMAs
 constexpr int THREADS = 32 * (SW + DW + 1);
 constexpr float P_EXP = 6.0f, SLACK = 8.0f;   // p is held times 2^6, and up to 2^14: fp16 reaches 2^16
@@ -71,6 +70,7 @@ __global__ void __launch_bounds__(512) k_kvq_scan(AttnKvqArgs a, int* marks, int
     unsigned top[2] = {0, 0};
     if (si.tiles) {
         const long long n = (si.len + 15) / 16 * parts;
+#pragma unroll 4
         for (long long x = threadIdx.x; x < n; x += blockDim.x) {
             const int gi = (int)(x / parts), part = (int)(x - (long long)gi * parts), pi = gi / gpp;
             const int page = a.b.table[(size_t)b * a.b.max_pages + pi];
@@ -115,12 +115,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     using T = typename Elem<DT>::T;
     const AttnKvqArgs& a = t.a;
     constexpr int HD = 32 * NB, ATOM = QT * 128;               // bytes of 64 dimensions of 128 rows
-    constexpr int Q_BYTES = NB / 2 * ATOM, SLOT = 8192 * NB, V_ATOM = HD * 128;
+    constexpr int Q_BYTES = NB / 2 * ATOM, SLOT = 4096 * NB, K_ATOM = TK * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t q_full, full[SLOTS], empty[SLOTS], s_full[2], p_ready[2], o_full[2];
+    __shared__ __align__(8) uint64_t q_full, full[SLOTS], empty[SLOTS], s_full[2][2], p_ready[2][2], pv_done[2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
-    __shared__ __align__(4) uint8_t s_valid[4][DW];   // [tile % 4][conversion warp]: bits of its two granules
+    __shared__ __align__(4) uint8_t s_valid[8][DW];   // [tile % 8][conversion warp]: whether its granule exists
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = blockIdx.y, b = blockIdx.z;
 
@@ -139,7 +139,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     if (tid == 0) {
         mbar_init(&q_full, 32 * SW);
         for (int i = 0; i < SLOTS; i++) mbar_init(&full[i], 32 * DW), mbar_init(&empty[i], 1);
-        for (int i = 0; i < 2; i++) mbar_init(&s_full[i], 1), mbar_init(&p_ready[i], QT), mbar_init(&o_full[i], 1);
+        for (int i = 0; i < 2; i++) {
+            for (int x = 0; x < 2; x++) mbar_init(&s_full[i][x], 1), mbar_init(&p_ready[i][x], QT);
+            mbar_init(&pv_done[i], 1);
+        }
         s_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;");
     }
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = s_tmem;   // S (and P) of tile q at 128 q, O at 256 + 128 q
+    const uint32_t tmem = s_tmem;   // S (and P) of query tile q at 128 q + 64 (tile & 1), O at 256 + 128 q
     volatile int* failed = &s_failed;
 
     if (warp < SW) {
@@ -202,73 +205,65 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
         float m = -INFINITY, off = 0.0f, l = 0.0f;
         bool good = true;
         for (int i = 0; i < tiles && good; i++) {
-            good = __all_sync(0xffffffffu, mbar_wait(&s_full[q], i & 1, failed));
+            good = __all_sync(0xffffffffu, mbar_wait(&s_full[q][i & 1], i >> 1 & 1, failed));
             if (!good) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t have = *reinterpret_cast<const volatile uint32_t*>(s_valid[i & 3]);   // two bits a byte
+            const uint32_t have = *reinterpret_cast<const volatile uint32_t*>(s_valid[i & 7]), s_i = s_at + (i & 1) * TK;
             const int t0 = i * TK;
-            const bool edge = t0 + TK > lim_min || have != 0x03030303u;
-            auto hidden = [&](int c) {   // whether the row attends to the tile's token c
-                return t0 + c >= lim || !(have >> (c / 32 * 8 + c / 16 % 2) & 1);
-            };
-            float top = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < TK; c += 32) {
-                uint32_t v[32];
-                tmem_ld<32>(v, s_at + c);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (edge) {
+            uint32_t v[2][32];
+            tmem_ld<32>(v[0], s_i);
+            tmem_ld<32>(v[1], s_i + 32);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            const bool edge = t0 + TK > lim_min || have != 0x01010101u;
+            if (edge) {
 #pragma unroll
-                    for (int x = 0; x < 32; x++)
-                        if (!hidden(c + x)) top = fmaxf(top, __uint_as_float(v[x]));
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 32; x++) top = fmaxf(top, __uint_as_float(v[x]));
-                }
+                for (int x = 0; x < TK; x++)   // hidden from the row, or not in the cache
+                    if (t0 + x >= lim || !(have >> (x / 16 * 8) & 1)) v[x / 32][x % 32] = __float_as_uint(-INFINITY);
             }
+            float top = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < TK; x++) top = fmaxf(top, __uint_as_float(v[x / 32][x % 32]));
             top = top == -INFINITY ? top : top * fac;
             if (__any_sync(0xffffffffu, top > m + SLACK)) {
                 const float mn = fmaxf(m, top), f = mn == m ? 1.0f : ex2(m - mn);
                 m = mn;
                 off = m == -INFINITY ? 0.0f : P_EXP - m;
                 l *= f;
-                if (i) {   // S of this tile was issued behind the last O += P V, so O is at rest
+                if (i) {
+                    good = __all_sync(0xffffffffu, mbar_wait(&pv_done[q], (i - 1) & 1, failed));   // O is at rest
+                    if (!good) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 32) {
-                        uint32_t v[32];
-                        tmem_ld<32>(v, o_at + c);
+                        uint32_t w[32];
+                        tmem_ld<32>(w, o_at + c);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                        for (int x = 0; x < 32; x++) v[x] = __float_as_uint(__uint_as_float(v[x]) * f);
-                        tmem_st(o_at + c, v);
+                        for (int x = 0; x < 32; x++) w[x] = __float_as_uint(__uint_as_float(w[x]) * f);
+                        tmem_st(o_at + c, w);
                     }
                 }
             }
-#pragma unroll 1
-            for (int c = 0; c < TK; c += 32) {
-                uint32_t v[32], p[16];
-                tmem_ld<32>(v, s_at + c);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            uint32_t p[32];
+            float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-                for (int x = 0; x < 32; x++) v[x] = __float_as_uint(ex2(fmaf(__uint_as_float(v[x]), fac, off)));
-                if (edge) {
+            for (int x = 0; x < 32; x++) {
+                float y[2];
 #pragma unroll
-                    for (int x = 0; x < 32; x++)
-                        if (hidden(c + x)) v[x] = 0u;
+                for (int z = 0; z < 2; z++) {
+                    const float s = __uint_as_float(v[x / 16][2 * (x % 16) + z]);
+                    y[z] = ex2(fmaf(s, fac, off));
+                    sum[z] += y[z];
                 }
-#pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    const float p0 = __uint_as_float(v[2 * x]), p1 = __uint_as_float(v[2 * x + 1]);
-                    l += p0 + p1;
-                    p[x] = as_u32(__floats2half2_rn(p0, p1));
-                }
-                tmem_st(s_at + c / 2, p);   // over scores that have been read
+                p[x] = as_u32(__floats2half2_rn(y[0], y[1]));
             }
+            l += sum[0] + sum[1];
+            tmem_st(s_i, p);   // over scores that have been read
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            mbar_arrive(&p_ready[q]);
+            mbar_arrive(&p_ready[q][i & 1]);
         }
-        if (good && tiles) good = __all_sync(0xffffffffu, mbar_wait(&o_full[q], 0, failed));
+        if (good && tiles) good = __all_sync(0xffffffffu, mbar_wait(&pv_done[q], (tiles - 1) & 1, failed));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inv = !good ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
         const float v2 = pow2(ex.y);
@@ -295,69 +290,64 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             }
         }
     } else if (warp < SW + DW) {
-        // ================================ codes into operands: two granules of each tile per warp
+        // ================================ codes into operands: a granule of each tile per warp
         const int dw = warp - SW, g = lane >> 2, c = lane & 3, gpp = a.c.pt >> 4;
         const __half2 kmul = __float2half2_rn(pow2(-ex.x)), vmul = __float2half2_rn(pow2(-ex.y));
         const uint32_t k1024 = a.k1024;
-        uint32_t kw[2][2][NB], vw[2][2][NB], ks[2][2][NB / 2], vs[2][2][NB];   // [granule][half]
-        const uint8_t* at[2];
-        uint32_t valid = 0;
-        auto find = [&](int i) {   // the tile's two granules; none behind the last row that is seen
-            valid = 0;
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const int gi = i * (TK / 16) + 2 * dw + x;
-                at[x] = nullptr;
-                if (gi * 16 >= seen) {
-                    valid |= 1u << x;   // hidden by the rows' limits
-                    continue;
-                }
-                const int pi = gi / gpp, page = a.b.table[(size_t)b * a.b.max_pages + pi];
-                if (page < 0 || page >= a.c.n_pages) {
-                    if (lane == 0) kvq_flag(a.b, TGX_KVQ_BAD_PAGE);
-                    continue;
-                }
-                valid |= 1u << x;
-                at[x] = kvq_granule(a.c, page, j, (gi - pi * gpp) * 16);
-            }
+        uint32_t kw[2][NB], vw[2][NB], ks[2][NB / 2], vs[2][NB];   // [half]
+        const uint8_t* at = nullptr;
+        bool there = true;
+        auto find = [&](int i) {   // the tile's granule; none behind the last row that is seen
+            const int gi = i * (TK / 16) + dw;
+            at = nullptr;
+            there = true;
+            if (gi * 16 >= seen) return;   // hidden by the rows' limits
+            const int pi = gi / gpp, page = a.b.table[(size_t)b * a.b.max_pages + pi];
+            there = page >= 0 && page < a.c.n_pages;
+            if (there)
+                at = kvq_granule(a.c, page, j, (gi - pi * gpp) * 16);
+            else if (lane == 0)
+                kvq_flag(a.b, TGX_KVQ_BAD_PAGE);
         };
         auto load_k = [&] {
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+            for (int h = 0; h < 2; h++) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int y = 0; y < NB; y++) kw[h][y] = 0;
 #pragma unroll
-                    for (int y = 0; y < NB; y++) kw[x][h][y] = 0;
-#pragma unroll
-                    for (int y = 0; y < NB / 2; y++) ks[x][h][y] = 0;
-                    if (at[x]) {
-                        load_words<NB>(kw[x][h], at[x] + (h * 32 + lane) * NB * 4);
-                        load_words<NB / 2>(ks[x][h], at[x] + 16 * HD + (h * 8 + g) * NB * 2);
-                    }
+                for (int y = 0; y < NB / 2; y++) ks[h][y] = 0;
+                if (at) {
+                    load_words<NB>(kw[h], at + (h * 32 + lane) * NB * 4);
+                    load_words<NB / 2>(ks[h], at + 16 * HD + (h * 8 + g) * NB * 2);
                 }
+            }
         };
         auto load_v = [&](int i) {
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+            for (int h = 0; h < 2; h++) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int y = 0; y < NB; y++) vw[h][y] = vs[h][y] = 0;
+                if (at) {
+                    load_words<NB>(vw[h], at + 8 * HD + (h * 32 + lane) * NB * 4);
+                    load_words<NB>(vs[h], at + 17 * HD + (h * 4 + c) * NB * 4);
+                    // rows behind the last hold anything
+                    const long long left = si.len - (i * TK + dw * 16 + 8 * h + 2 * c);
+                    if (left < 2)
 #pragma unroll
-                    for (int y = 0; y < NB; y++) vw[x][h][y] = vs[x][h][y] = 0;
-                    if (at[x]) {
-                        load_words<NB>(vw[x][h], at[x] + 8 * HD + (h * 32 + lane) * NB * 4);
-                        load_words<NB>(vs[x][h], at[x] + 17 * HD + (h * 4 + c) * NB * 4);
-                        // rows behind the last hold anything
-                        const long long left = si.len - (i * TK + (2 * dw + x) * 16 + 8 * h + 2 * c);
-                        if (left < 2)
-#pragma unroll
-                            for (int y = 0; y < NB; y++) vs[x][h][y] &= left == 1 ? 0xffffu : 0u;
-                    }
+                        for (int y = 0; y < NB; y++) vs[h][y] &= left == 1 ? 0xffffu : 0u;
                 }
+            }
         };
         int slot = 0;
         uint32_t phase = 1;   // of `empty`: a fresh barrier's wait for it passes
         auto next = [&] {
             if (++slot == SLOTS) slot = 0, phase ^= 1;
+        };
+        // the lane's four code pairs of a word
+        auto codes = [&](uint32_t (&z)[4], uint32_t w) {
+            const uint32_t x = w >> 8;
+            z[0] = codes_lo<false>(w, k1024), z[1] = codes_hi<false>(w, k1024);
+            z[2] = codes_lo<false>(x, k1024), z[3] = codes_hi<false>(x, k1024);
         };
         bool good = true;
         if (tiles) {
@@ -366,28 +356,24 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
         }
         for (int i = 0; i < tiles; i++) {
             load_v(i);
-            if (lane == 0) s_valid[i & 3][dw] = (uint8_t)valid;
+            if (lane == 0) s_valid[i & 7][dw] = there ? 1 : 0;
             good = mbar_wait(&empty[slot], phase, failed);
             if (!good) break;
             uint8_t* to = ring + slot * SLOT;
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+            for (int h = 0; h < 2; h++) {
+                uint8_t* row = to + (dw * 16 + 8 * h + g) * 128 + 4 * c;
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int row = (2 * dw + x) * 16 + 8 * h + g;
+                for (int y = 0; y < NB; y++) {
+                    const __half2 pair = as_h2(ks[h][y / 2]);
+                    const __half2 d = __hmul2(y & 1 ? __high2half2(pair) : __low2half2(pair), kmul);
+                    uint32_t z[4];
+                    codes(z, kw[h][y]);
 #pragma unroll
-                    for (int y = 0; y < NB; y++) {
-                        const uint32_t w = kw[x][h][y];
-                        const __half2 pair = as_h2(ks[x][h][y / 2]);
-                        const __half2 d = __hmul2(y & 1 ? __high2half2(pair) : __low2half2(pair), kmul);
-                        const uint32_t z[4] = {codes_lo<false>(w, k1024), codes_hi<false>(w, k1024),
-                                               codes_lo<false>(w >> 8, k1024), codes_hi<false>(w >> 8, k1024)};
-#pragma unroll
-                        for (int n = 0; n < 4; n++)
-                            *reinterpret_cast<uint32_t*>(to + y / 2 * ATOM + row * 128 + (((y % 2) * 4 + n) ^ g) * 16 + 4 * c) =
-                                as_u32(__hmul2(as_h2(z[n]), d));
-                    }
+                    for (int n = 0; n < 4; n++)
+                        *reinterpret_cast<uint32_t*>(row + y / 2 * K_ATOM + (((y % 2) * 4 + n) ^ g) * 16) = as_u32(__hmul2(as_h2(z[n]), d));
                 }
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(&full[slot]);
             next();
@@ -399,74 +385,85 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             if (!good) break;
             to = ring + slot * SLOT;
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+            for (int h = 0; h < 2; h++) {
+                uint8_t* row = to + g * 128 + ((dw * 2 + h) ^ g) * 16 + 4 * c;   // 16 bytes: 8 tokens
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int gr = 2 * dw + x, chunk = (gr % 4) * 2 + h;   // 16 bytes: 8 tokens
+                for (int y = 0; y < NB; y++) {
+                    const __half2 d = __hmul2(as_h2(vs[h][y]), vmul);
+                    uint32_t z[4];
+                    codes(z, vw[h][y]);
 #pragma unroll
-                    for (int y = 0; y < NB; y++) {
-                        const uint32_t w = vw[x][h][y];
-                        const __half2 d = __hmul2(as_h2(vs[x][h][y]), vmul);
-                        const uint32_t z[4] = {codes_lo<false>(w, k1024), codes_hi<false>(w, k1024),
-                                               codes_lo<false>(w >> 8, k1024), codes_hi<false>(w >> 8, k1024)};
-#pragma unroll
-                        for (int n = 0; n < 4; n++)
-                            *reinterpret_cast<uint32_t*>(to + gr / 4 * V_ATOM + (32 * y + 8 * n + g) * 128 + (chunk ^ g) * 16 + 4 * c) =
-                                as_u32(__hmul2(as_h2(z[n]), d));
-                    }
+                    for (int n = 0; n < 4; n++)
+                        *reinterpret_cast<uint32_t*>(row + (32 * y + 8 * n) * 128) = as_u32(__hmul2(as_h2(z[n]), d));
                 }
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(&full[slot]);
             next();
         }
-    } else if (lane == 0 && tiles) {
+    } else if (tiles) {
         // ================================ the MMAs
         constexpr uint32_t IDESC_S = (1u << 4) | ((TK >> 3) << 17) | ((QT >> 4) << 24);
         constexpr uint32_t IDESC_O = (1u << 4) | ((HD >> 3) << 17) | ((QT >> 4) << 24);
         const uint64_t dq = sw128_desc(saddr(s_q)), dr = sw128_desc(saddr(ring));
-        auto scores = [&](int q, int slot) {
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        // the warp is in step throughout; one lane issues
+        auto scores = [&](int q, int i, int slot, bool last) {
+            const uint32_t d = tm + q * 128 + (i & 1) * TK;
+            const uint64_t x = dq + (q * Q_BYTES >> 4), y = dr + (slot * SLOT >> 4);
+            if (elect_one()) {
 #pragma unroll
-            for (int s = 0; s < 2 * NB; s++)
-                mma_f16_ss(tmem + q * 128, dq + ((q * Q_BYTES + s / 4 * ATOM + s % 4 * 32) >> 4),
-                           dr + ((slot * SLOT + s / 4 * ATOM + s % 4 * 32) >> 4), IDESC_S, s > 0);
+                for (int s = 0; s < 2 * NB; s++)
+                    mma_f16_ss(d, x + ((s / 4 * ATOM + s % 4 * 32) >> 4), y + ((s / 4 * K_ATOM + s % 4 * 32) >> 4), IDESC_S, s > 0);
+                commit(&s_full[q][i & 1]);
+                if (last) commit(&empty[slot]);
+            }
+            __syncwarp();
         };
-        auto values = [&](int q, int slot, bool add) {
+        auto values = [&](int q, int i, int slot, bool last) {
+            const uint32_t d = tm + 256 + q * 128, x = tm + q * 128 + (i & 1) * TK;
+            const uint64_t y = dr + (slot * SLOT >> 4);
+            if (elect_one()) {
 #pragma unroll
-            for (int s = 0; s < TK / 16; s++)
-                mma_f16_ts(tmem + 256 + q * 128, tmem + q * 128 + 8 * s, dr + ((slot * SLOT + s / 4 * V_ATOM + s % 4 * 32) >> 4),
-                           IDESC_O, add || s > 0);
+                for (int s = 0; s < TK / 16; s++) mma_f16_ts(d, x + 8 * s, y + (s * 32 >> 4), IDESC_O, i > 0 || s > 0);
+                commit(&pv_done[q]);
+                if (last) commit(&empty[slot]);
+            }
+            __syncwarp();
         };
         auto fence = [] { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); };
-        bool good = mbar_wait(&q_full, 0, failed) && mbar_wait(&full[0], 0, failed);
+        int kslot = 0, vslot = 1;                // of K of the next tile, and V of this one
+        uint32_t kphase = 0, vphase = 0;
+        auto step = [](int& slot, uint32_t& phase) {
+            slot += 2;
+            if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
+        };
+        auto wait = [&](uint64_t* m, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(m, parity, failed)); };
+        bool good = wait(&q_full, 0) && wait(&full[0], 0);
         if (good) {
             fence();
-            scores(0, 0);
-            commit(&s_full[0]);
-            scores(1, 0);
-            commit(&s_full[1]);
-            commit(&empty[0]);
+            scores(0, 0, 0, false);
+            scores(1, 0, 0, true);
+            step(kslot, kphase);
         }
-        for (int i = 0, f = 1; i < tiles && good; i++, f += 2) {   // V of tile i is the ring's f'th, K of the next f + 1'th
-            const int vslot = f % SLOTS, kslot = (f + 1) % SLOTS;
+        for (int i = 0; i < tiles && good; i++) {
             const bool more = i + 1 < tiles;
-            good = mbar_wait(&full[vslot], f / SLOTS & 1, failed) && (!more || mbar_wait(&full[kslot], (f + 1) / SLOTS & 1, failed));
+            if (more) good = wait(&full[kslot], kphase);
             for (int q = 0; q < 2 && good; q++) {
-                good = mbar_wait(&p_ready[q], i & 1, failed);
+                if (more) {   // the next scores go into the other half of S, which O's last sum has read
+                    fence();
+                    scores(q, i + 1, kslot, q == 1);
+                }
+                good = (q || wait(&full[vslot], vphase)) && wait(&p_ready[q][i & 1], i >> 1 & 1);
                 if (!good) break;
                 fence();
-                values(q, vslot, i > 0);
-                if (q == 1) commit(&empty[vslot]);
-                if (more) {
-                    scores(q, kslot);
-                    commit(&s_full[q]);
-                    if (q == 1) commit(&empty[kslot]);
-                } else {
-                    commit(&o_full[q]);
-                }
+                values(q, i, vslot, q == 1);
             }
+            step(kslot, kphase);
+            step(vslot, vphase);
         }
         if (!good) {   // what is under way ends before the TMEM is freed: one more commit behind it all
-            commit(&q_full);
+            if (elect_one()) commit(&q_full);
             const long long t0 = clock64();
             while (!mbar_try(&q_full, 1) && clock64() - t0 < WAIT_CYCLES / 16) {
             }
@@ -482,7 +479,7 @@ size_t r256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 template <int DT, int NB>
 cudaError_t launch_tc(const TcArgs& t, cudaStream_t s) {
-    constexpr int smem = 2 * (NB / 2) * QT * 128 + SLOTS * 8192 * NB + 1024;
+    constexpr int smem = 2 * (NB / 2) * QT * 128 + SLOTS * 4096 * NB + 1024;
     cudaError_t e = cudaFuncSetAttribute(k_kvq_tc<DT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const long long rows = (long long)t.a.b.max_new * t.a.R;

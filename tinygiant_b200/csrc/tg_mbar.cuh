@@ -47,6 +47,15 @@ __device__ __forceinline__ void mbar_drain(uint64_t* m, uint32_t parity) {
     }
 }
 
+// One lane of the warp, the same every time.  The instructions of tcgen05 take their operands from
+// uniform registers: with a warp in step around this, descriptors stay there, while a branch on
+// the lane's number has every one moved over first (a third of the rate, measured).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes;
+}
+
 // K-major operand in 128-byte swizzle: rows of 128 bytes, 8-row atoms 1024 bytes apart.
 __device__ __forceinline__ uint64_t sw128_desc(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
