@@ -940,8 +940,8 @@ template <int DT>
 cudaError_t launch_t(const AttnKvqArgs& a, void* scratch, size_t n, cudaStream_t s) { TG_NB(DT, launch_attn_nb, a, scratch, n, s) }
 
 cudaError_t launch_attn(int dtype, AttnKvqArgs a, void* scratch, size_t n, cudaStream_t s) {
-    if (attn_tc_takes(dtype, a.c, a.b, a.R)) {
-        const size_t tc = attn_tc_scratch(a.c, a.b);
+    if (attn_tc_takes(dtype, a.c, a.b, a.T, a.R)) {
+        const size_t tc = attn_tc_scratch(a.c, a.b, a.T, a.R);
         if (n < tc) return cudaErrorInvalidValue;
         cudaError_t e = launch_attn_tc(dtype, a, scratch, &a.only, s);
         if (e != cudaSuccess) return e;
@@ -969,7 +969,7 @@ extern "C" size_t tgx_kvq_attention_scratch_bytes(const tgx_kvq_cache* cache, co
     for (int two = 0; two < 2; two++)
         most = std::max(most, tg::attn_scratch(tg::shape_of(c, b, n_heads / c.nkv, two, tg::MAX_SMS * tg::workers_per_sm(1),
                                                             tg::MAX_SMS * tg::workers_per_sm(tg::DEEP_WARPS)), c.hd));
-    return most + tg::attn_tc_scratch(c, b);
+    return most + tg::attn_tc_scratch(c, b, n_tokens, n_heads / c.nkv);
 }
 
 extern "C" int tgx_kvq_attention(const tgx_kvq_cache* cache, const tgx_kvq_batch* batch, int dtype, int n_tokens,

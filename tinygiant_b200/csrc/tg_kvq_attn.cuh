@@ -120,8 +120,8 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnKvqArgs& a, int b, int til
 // The 256-row tiles of tg_kvq_tc.cu: whether they take the call, their scratch, and the launch
 // (which leaves sequences with a scale that is not finite, marked in its scratch, to the other
 // kernel: *only then points at the marks).
-bool attn_tc_takes(int dtype, const KvqCache& c, const KvqBatch& b, int R);
-size_t attn_tc_scratch(const KvqCache& c, const KvqBatch& b);
+bool attn_tc_takes(int dtype, const KvqCache& c, const KvqBatch& b, int T, int R);
+size_t attn_tc_scratch(const KvqCache& c, const KvqBatch& b, int T, int R);
 cudaError_t launch_attn_tc(int dtype, const AttnKvqArgs& a, void* scratch, const int** only, cudaStream_t s);
 
 }  // namespace tg

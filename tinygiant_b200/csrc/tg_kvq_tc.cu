@@ -6,7 +6,7 @@
 //   S = Q K^T     kind::f16, 128 x 64 fp32 in TMEM, two of them per query tile
 //   p = 2^(s - m) a thread per query row, reading its TMEM lane; P goes back over S as fp16
 //   O += P V      A from TMEM, B the transposed V tile
-// Codes are turned into fp16 values once per CTA and tile, code * d rounded to 11 bits, by four
+// Codes are turned into fp16 values once per CTA and tile, code * d rounded to 11 bits, by eight
 // warps that read the granules straight into registers (the next tile's while this one's are
 // converted) and write the 128-byte-swizzled operands; a ring of six slots holds K, V, K, ...
 // The layout of the cache makes both K-major operands of 4-byte pieces that 32 lanes store
@@ -30,16 +30,18 @@ namespace tg {
 namespace {
 
 constexpr int QT = 128;          // query rows of a tile
-constexpr int TK = 64;           // tokens of a tile: a granule per conversion warp
+constexpr int TK = 64;           // tokens of a tile: half a granule per conversion warp
 constexpr int SLOTS = 6;
-constexpr int SW = 8, DW = 4;    // softmax and conversion warps; one more for the MMAs
-constexpr int THREADS = 32 * (SW + DW + 1);
+constexpr int SW = 8, DW = 8;    // softmax and conversion warps; one more for the MMAs
+constexpr int THREADS = 32 * (SW + DW + 4);
 constexpr float P_EXP = 6.0f, SLACK = 8.0f;   // p is held times 2^6, and up to 2^14: fp16 reaches 2^16
 
 struct TcArgs {
     AttnKvqArgs a;
     const int* marks;      // [B][nkv]
     const int2* exps;      // [B][nkv] exponents of K and V
+    const int2* order;     // the items (sequence, tile of 256 rows) by the rows they see, the most first
+    const int* items;      // how many
 };
 
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
@@ -56,41 +58,70 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
 __device__ __forceinline__ void commit(uint64_t* m) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(m)) : "memory");
 }
+// The exponent by which a row of q is divided, from its largest magnitude.
+__device__ __forceinline__ int q_exp(unsigned top) {
+    const int field = (int)(top >> 23);
+    return field == 255 || top == 0 ? 0 : max(field - 127, -100) - 13;
+}
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }   // -126 .. 127
 
+// Rows of the cache that the last row of tile rt sees.
+__device__ __forceinline__ int item_seen(const AttnKvqArgs& a, const SeqInfo& si, int rt) {
+    const int last = min((rt + 1) * 2 * QT, si.n * a.R) - 1;
+    return (int)max(0ll, min(si.len, (long long)si.off + last / a.R + 1));
+}
+
 // The largest scale magnitudes of every (sequence, kv head)'s cached rows as exponents, and whether
-// one of them is not finite.
-__global__ void __launch_bounds__(512) k_kvq_scan(AttnKvqArgs a, int* marks, int2* exps) {
+// one of them is not finite; and the order of the items: an item's place is the number of those
+// that see more.
+__global__ void __launch_bounds__(1024) k_kvq_scan(AttnKvqArgs a, int* marks, int2* exps, int2* order, int* items, int cap) {
     __shared__ unsigned s_top[2];
-    const int j = blockIdx.x, b = blockIdx.y, hd = a.c.hd, nb = hd / 32;
+    const int j = blockIdx.x, b = blockIdx.y, hd = a.c.hd, lb = hd == 128 ? 2 : 1;   // 2^lb blocks a row
     const SeqInfo si = seq_info(a, b, 2 * QT);
     if (threadIdx.x < 2) s_top[threadIdx.x] = 0;
     __syncthreads();
     const int parts = 2 * hd / 16, gpp = a.c.pt >> 4;   // 16-byte parts of a granule's scales: K's, then V's
     unsigned top[2] = {0, 0};
     if (si.tiles) {
-        const long long n = (si.len + 15) / 16 * parts;
-#pragma unroll 4
-        for (long long x = threadIdx.x; x < n; x += blockDim.x) {
-            const int gi = (int)(x / parts), part = (int)(x - (long long)gi * parts), pi = gi / gpp;
-            const int page = a.b.table[(size_t)b * a.b.max_pages + pi];
-            if (page < 0 || page >= a.c.n_pages) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(kvq_granule(a.c, page, j, (gi - pi * gpp) * 16) + 16 * hd + 16 * part);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            const bool is_v = part >= hd / 16;
-            const int left = (int)min(16ll, si.len - 16ll * gi);   // tokens of the granule
-            unsigned most = 0;
+        // a granule's parts are neighbouring threads'; four granules a thread at a time
+        const int per = (int)blockDim.x / parts, part = (int)threadIdx.x % parts, grans = (int)((si.len + 15) / 16);
+        const bool is_v = part >= hd / 16;
+        unsigned most = 0;
+        for (int g0 = (int)threadIdx.x / parts; g0 < grans && (int)threadIdx.x < per * parts; g0 += 4 * per) {
+            uint4 v[4];
+            int page[4];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int at = (is_v ? part - hd / 16 : part) * 8 + i;   // which half of K's or V's
-                // V's pairs: [h][c][block][e]
-                const int tok = is_v ? at / (2 * nb) * 2 + (at & 1) : at / nb;
-                const unsigned u = w[i / 2] >> (16 * (i & 1)) & 0x7fffu;
-                if (tok < left) most = max(most, u);
+            for (int y = 0; y < 4; y++) {
+                const int gi = g0 + y * per;
+                page[y] = gi < grans ? a.b.table[(size_t)b * a.b.max_pages + gi / gpp] : -1;
             }
-            top[0] = is_v ? top[0] : max(top[0], most);
-            top[1] = is_v ? max(top[1], most) : top[1];
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const int gi = g0 + y * per;
+                v[y] = make_uint4(0, 0, 0, 0);
+                if (page[y] >= 0 && page[y] < a.c.n_pages)
+                    v[y] = *reinterpret_cast<const uint4*>(kvq_granule(a.c, page[y], j, gi % gpp * 16) + 16 * hd + 16 * part);
+            }
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const uint32_t w[4] = {v[y].x, v[y].y, v[y].z, v[y].w};
+                const long long left = si.len - 16ll * (g0 + y * per);   // tokens of the granule
+                if (left >= 16) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) most = max(most, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
+                    continue;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int at = (is_v ? part - hd / 16 : part) * 8 + i;   // which half of K's or V's
+                    // V's pairs: [h][c][block][e]
+                    const int tok = is_v ? (at >> (1 + lb)) * 2 + (at & 1) : at >> lb;
+                    if (tok < left) most = max(most, w[i / 2] >> (16 * (i & 1)) & 0x7fffu);
+                }
+            }
         }
+        top[0] = is_v ? 0 : most;
+        top[1] = is_v ? most : 0;
     }
 #pragma unroll
     for (int i = 0; i < 2; i++) {
@@ -98,6 +129,29 @@ __global__ void __launch_bounds__(512) k_kvq_scan(AttnKvqArgs a, int* marks, int
         if ((threadIdx.x & 31) == 0) atomicMax(&s_top[i], top[i]);
     }
     __syncthreads();
+    if (j == 0) {   // a warp per item
+        const int lane = threadIdx.x & 31, rt_step = blockDim.x / 32;
+        for (int rt = threadIdx.x / 32; rt < si.tiles || (b == 0 && rt == threadIdx.x / 32); rt += rt_step) {
+            const int mine = rt < si.tiles ? item_seen(a, si, rt) : 0;
+            int rank = 0, all = 0;
+            for (int x = lane; x < a.b.B; x += 32) {
+                const SeqInfo sx = seq_info(a, x, 2 * QT);
+                int lo = 0, hi = sx.tiles;   // the first that is in front of mine: they see more and more
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1, see = item_seen(a, sx, mid);
+                    const bool front = see > mine || (see == mine && (x < b || (x == b && mid > rt)));
+                    if (front)
+                        hi = mid;
+                    else
+                        lo = mid + 1;
+                }
+                rank += sx.tiles - lo, all += sx.tiles;
+            }
+            rank = __reduce_add_sync(0xffffffffu, rank), all = __reduce_add_sync(0xffffffffu, all);
+            if (lane == 0 && rt < si.tiles && rank < cap) order[rank] = make_int2(b, rt);
+            if (threadIdx.x == 0 && b == 0) *items = min(all, cap);   // more than cap: q_start goes back
+        }
+    }
     if (threadIdx.x == 0) {
         int e[2];
 #pragma unroll
@@ -120,13 +174,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     __shared__ __align__(8) uint64_t q_full, full[SLOTS], empty[SLOTS], s_full[2][2], p_ready[2][2], pv_done[2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
-    __shared__ __align__(4) uint8_t s_valid[8][DW];   // [tile % 8][conversion warp]: whether its granule exists
+    __shared__ __align__(4) uint8_t s_valid[8][TK / 16];   // [tile % 8]: whether its granules exist
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = blockIdx.y, b = blockIdx.z;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    const int item = blockIdx.x / a.c.nkv, j = blockIdx.x % a.c.nkv;   // the longest first
+    if (item >= *t.items) return;
+    const int b = t.order[item].x, rt = t.order[item].y;
     const SeqInfo si = seq_info(a, b, 2 * QT);
-    const int rt = si.tiles - 1 - (int)blockIdx.x;   // the longest first
-    if (rt < 0) return;
     for (int x = 0; x < a.c.nkv; x++)
         if (t.marks[b * a.c.nkv + x]) return;
     const int row0 = rt * 2 * QT, nrows = min(2 * QT, si.n * a.R - row0);
@@ -156,46 +211,59 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     const uint32_t tmem = s_tmem;   // S (and P) of query tile q at 128 q + 64 (tile & 1), O at 256 + 128 q
     volatile int* failed = &s_failed;
 
+    // 640 threads start with 96 registers each (61440): 256 x 128 + 256 x 80 + 128 x 64 are as many
     if (warp < SW) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         // ================================ a thread per query row
         const int q = warp >> 2, r = (warp & 3) * 32 + lane, x0 = q * QT;
         const bool ok = x0 + r < nrows;
-        const int rho = row0 + x0 + (ok ? r : 0);
+        const int rho = row0 + (ok ? x0 + r : 0);   // rows behind the last are the item's first, and not written back
         const int lim = ok ? limit(rho / a.R) : 0x7fffffff;
         const int lim_min = x0 < nrows ? limit((row0 + x0) / a.R) : 0x7fffffff;
+        constexpr int RPI = 128 / HD, LPR = 32 / RPI;   // rows that a warp reads at once, 4 elements a lane
+        const int lr = lane / LPR, ld = lane % LPR * 4; // its row of those, and dimension
+        uint8_t* const s_row = s_q + q * Q_BYTES + (r - lane) * 128;   // rows of this warp
+        auto piece = [&](int row) { return s_row + row * 128 + ld / 64 * ATOM + ((ld % 64 / 8) ^ (row & 7)) * 16 + (ld & 4) * 2; };
+        auto row_at = [&](long long stride) {   // of the thread's row of q or out
+            return (si.s0 + rho / a.R) * stride + (j * a.R + rho % a.R) * HD;
+        };
+        struct alignas(4 * sizeof(T)) Vec { T t[4]; };
         float fac;
         {
-            const T* src = reinterpret_cast<const T*>(a.q) + (size_t)(si.s0 + rho / a.R) * a.qs + (size_t)(j * a.R + rho % a.R) * HD;
-            auto load4 = [&](float (&v)[4], int d) {
-                struct alignas(4 * sizeof(T)) Vec { T t[4]; };
-                const Vec u = *reinterpret_cast<const Vec*>(src + d);
+            unsigned top = 0;
+            const int lr = lane / LPR, ld = lane % LPR * 4;   // the lane's row of those, and dimension
+            const long long at = row_at(a.qs);
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = ok ? to_f32(u.t[i]) : 0.0f;
-            };
-            float top = 0.0f;
-#pragma unroll 8
-            for (int d = 0; d < HD; d += 4) {
-                float v[4];
-                load4(v, d);
-                top = fmaxf(fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+            for (int y0 = 0; y0 < LPR; y0 += 16) {
+                Vec u[16];
+#pragma unroll
+                for (int y = 0; y < 16; y++)
+                    u[y] = *reinterpret_cast<const Vec*>(reinterpret_cast<const T*>(a.q) + __shfl_sync(0xffffffffu, at, (y0 + y) * RPI + lr) + ld);
+#pragma unroll
+                for (int y = 0; y < 16; y++) {
+                    const int row = (y0 + y) * RPI + lr;
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] = to_f32(u[y].t[i]);
+                    unsigned most = __float_as_uint(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+                    if (RPI == 1) {
+                        most = __reduce_max_sync(0xffffffffu, most);
+                    } else {
+#pragma unroll
+                        for (int x = 1; x < LPR; x *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
+                    }
+                    // 2^-e: the largest into 2^13 .. 2^14; in two factors, as e reaches beyond fp32's exponents
+                    const int e = q_exp(most), half = e / 2;
+                    const float up1 = pow2(-half), up2 = pow2(-(e - half));
+                    uint2 w;
+                    w.x = as_u32(__floats2half2_rn(v[0] * up1 * up2, v[1] * up1 * up2));
+                    w.y = as_u32(__floats2half2_rn(v[2] * up1 * up2, v[3] * up1 * up2));
+                    *reinterpret_cast<uint2*>(piece(row)) = w;
+                    most = __shfl_sync(0xffffffffu, most, lane % RPI * LPR);
+                    if (lane / RPI == y0 + y) top = most;   // of the thread's own row
+                }
             }
-            // 2^-e: the largest into 2^13 .. 2^14; in two factors, as e reaches beyond fp32's exponents
-            const int field = (int)(__float_as_uint(top) >> 23);
-            const int e = field == 255 || top == 0.0f ? 0 : max(field - 127, -100) - 13, half = e / 2;
-            const float up1 = pow2(-half), up2 = pow2(-(e - half));
-            uint8_t* to = s_q + q * Q_BYTES + r * 128;
-#pragma unroll 4
-            for (int d = 0; d < HD; d += 8) {
-                float v[4], w[4];
-                load4(v, d);
-                load4(w, d + 4);
-                uint4 u;
-                u.x = as_u32(__floats2half2_rn(v[0] * up1 * up2, v[1] * up1 * up2));
-                u.y = as_u32(__floats2half2_rn(v[2] * up1 * up2, v[3] * up1 * up2));
-                u.z = as_u32(__floats2half2_rn(w[0] * up1 * up2, w[1] * up1 * up2));
-                u.w = as_u32(__floats2half2_rn(w[2] * up1 * up2, w[3] * up1 * up2));
-                *reinterpret_cast<uint4*>(to + d / 64 * ATOM + ((d % 64 / 8) ^ (r & 7)) * 16) = u;
-            }
+            const int e = q_exp(top), half = e / 2;
             fac = a.scale * pow2(half) * pow2(e - half) * pow2(ex.x);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(&q_full);
@@ -267,7 +335,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inv = !good ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
         const float v2 = pow2(ex.y);
-        T* dst = reinterpret_cast<T*>(a.out) + (size_t)(si.s0 + rho / a.R) * a.os + (size_t)(j * a.R + rho % a.R) * HD;
+        // through shared memory, where q is done with, so that a warp writes whole rows
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
             uint32_t v[32];
@@ -278,64 +346,52 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
 #pragma unroll
                 for (int x = 0; x < 32; x++) v[x] = 0u;
             }
-            if (ok) {
-                struct alignas(4 * sizeof(T)) Vec { T t[4]; };
 #pragma unroll
-                for (int x = 0; x < 32; x += 4) {
-                    Vec u;
+            for (int x = 0; x < 32; x += 8) {
+                struct alignas(16) Vec8 { T t[8]; } u;
 #pragma unroll
-                    for (int y = 0; y < 4; y++) from_f32(__uint_as_float(v[x + y]) * v2 * inv, u.t[y]);
-                    *reinterpret_cast<Vec*>(dst + c + x) = u;
-                }
+                for (int y = 0; y < 8; y++) from_f32(__uint_as_float(v[x + y]) * v2 * inv, u.t[y]);
+                *reinterpret_cast<Vec8*>(s_row + lane * 128 + c / 64 * ATOM + (((c + x) % 64 / 8) ^ (lane & 7)) * 16) = u;
             }
         }
+        __syncwarp();
+        const long long to = ok ? row_at(a.os) : -1;
+#pragma unroll 8
+        for (int y = 0; y < LPR; y++) {
+            const int row = y * RPI + lr;
+            const long long at = __shfl_sync(0xffffffffu, to, row);
+            if (at >= 0) *reinterpret_cast<Vec*>(reinterpret_cast<T*>(a.out) + at + ld) = *reinterpret_cast<const Vec*>(piece(row));
+        }
     } else if (warp < SW + DW) {
-        // ================================ codes into operands: a granule of each tile per warp
-        const int dw = warp - SW, g = lane >> 2, c = lane & 3, gpp = a.c.pt >> 4;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        // ================================ codes into operands: half a granule of each tile per warp
+        const int dw = warp - SW, gt = dw >> 1, h = dw & 1, g = lane >> 2, c = lane & 3, gpp = a.c.pt >> 4;
         const __half2 kmul = __float2half2_rn(pow2(-ex.x)), vmul = __float2half2_rn(pow2(-ex.y));
         const uint32_t k1024 = a.k1024;
-        uint32_t kw[2][NB], vw[2][NB], ks[2][NB / 2], vs[2][NB];   // [half]
-        const uint8_t* at = nullptr;
-        bool there = true;
-        auto find = [&](int i) {   // the tile's granule; none behind the last row that is seen
-            const int gi = i * (TK / 16) + dw;
-            at = nullptr;
-            there = true;
-            if (gi * 16 >= seen) return;   // hidden by the rows' limits
-            const int pi = gi / gpp, page = a.b.table[(size_t)b * a.b.max_pages + pi];
-            there = page >= 0 && page < a.c.n_pages;
-            if (there)
-                at = kvq_granule(a.c, page, j, (gi - pi * gpp) * 16);
-            else if (lane == 0)
-                kvq_flag(a.b, TGX_KVQ_BAD_PAGE);
+        struct Raw {
+            uint32_t kw[NB], ks[NB / 2], vw[NB], vs[NB];
+            bool there;
         };
-        auto load_k = [&] {
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-#pragma unroll
-                for (int y = 0; y < NB; y++) kw[h][y] = 0;
-#pragma unroll
-                for (int y = 0; y < NB / 2; y++) ks[h][y] = 0;
-                if (at) {
-                    load_words<NB>(kw[h], at + (h * 32 + lane) * NB * 4);
-                    load_words<NB / 2>(ks[h], at + 16 * HD + (h * 8 + g) * NB * 2);
-                }
-            }
+        auto page_of = [&](int i) -> int {   // the page of tile i's granule; 0 behind the last row that is seen
+            const int gi = i * (TK / 16) + gt;
+            return gi * 16 < seen ? a.b.table[(size_t)b * a.b.max_pages + gi / gpp] : 0;
         };
-        auto load_v = [&](int i) {
+        auto load = [&](Raw& x, int i, int page) {
+            const int gi = i * (TK / 16) + gt;
+            const bool in = gi * 16 < seen;   // what is not, the rows' limits hide
+            x.there = !in || (page >= 0 && page < a.c.n_pages);
+            if (!x.there && lane == 0) kvq_flag(a.b, TGX_KVQ_BAD_PAGE);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int y = 0; y < NB; y++) x.kw[y] = x.vw[y] = x.vs[y] = 0;
 #pragma unroll
-                for (int y = 0; y < NB; y++) vw[h][y] = vs[h][y] = 0;
-                if (at) {
-                    load_words<NB>(vw[h], at + 8 * HD + (h * 32 + lane) * NB * 4);
-                    load_words<NB>(vs[h], at + 17 * HD + (h * 4 + c) * NB * 4);
-                    // rows behind the last hold anything
-                    const long long left = si.len - (i * TK + dw * 16 + 8 * h + 2 * c);
-                    if (left < 2)
-#pragma unroll
-                        for (int y = 0; y < NB; y++) vs[h][y] &= left == 1 ? 0xffffu : 0u;
-                }
+            for (int y = 0; y < NB / 2; y++) x.ks[y] = 0;
+            if (in && x.there) {
+                const uint8_t* at = kvq_granule(a.c, page, j, gi % gpp * 16);
+                load_words<NB>(x.kw, at + (h * 32 + lane) * NB * 4);
+                load_words<NB / 2>(x.ks, at + 16 * HD + (h * 8 + g) * NB * 2);
+                load_words<NB>(x.vw, at + 8 * HD + (h * 32 + lane) * NB * 4);
+                load_words<NB>(x.vs, at + 17 * HD + (h * 4 + c) * NB * 4);
             }
         };
         int slot = 0;
@@ -349,123 +405,120 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             z[0] = codes_lo<false>(w, k1024), z[1] = codes_hi<false>(w, k1024);
             z[2] = codes_lo<false>(x, k1024), z[3] = codes_hi<false>(x, k1024);
         };
-        bool good = true;
+        Raw cur, nxt;
+        int page = 0;   // of the next tile
         if (tiles) {
-            find(0);
-            load_k();
+            load(cur, 0, page_of(0));
+            page = page_of(1);
         }
         for (int i = 0; i < tiles; i++) {
-            load_v(i);
-            if (lane == 0) s_valid[i & 7][dw] = there ? 1 : 0;
-            good = mbar_wait(&empty[slot], phase, failed);
-            if (!good) break;
-            uint8_t* to = ring + slot * SLOT;
+            load(nxt, i + 1, page);
+            page = page_of(i + 2);
+            if (lane == 0 && h == 0) s_valid[i & 7][gt] = cur.there ? 1 : 0;
+            if (!mbar_wait(&empty[slot], phase, failed)) break;
+            uint8_t* row = ring + slot * SLOT + (gt * 16 + 8 * h + g) * 128 + 4 * c;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint8_t* row = to + (dw * 16 + 8 * h + g) * 128 + 4 * c;
+            for (int y = 0; y < NB; y++) {
+                const __half2 pair = as_h2(cur.ks[y / 2]);
+                const __half2 d = __hmul2(y & 1 ? __high2half2(pair) : __low2half2(pair), kmul);
+                uint32_t z[4];
+                codes(z, cur.kw[y]);
 #pragma unroll
-                for (int y = 0; y < NB; y++) {
-                    const __half2 pair = as_h2(ks[h][y / 2]);
-                    const __half2 d = __hmul2(y & 1 ? __high2half2(pair) : __low2half2(pair), kmul);
-                    uint32_t z[4];
-                    codes(z, kw[h][y]);
-#pragma unroll
-                    for (int n = 0; n < 4; n++)
-                        *reinterpret_cast<uint32_t*>(row + y / 2 * K_ATOM + (((y % 2) * 4 + n) ^ g) * 16) = as_u32(__hmul2(as_h2(z[n]), d));
-                }
+                for (int n = 0; n < 4; n++)
+                    *reinterpret_cast<uint32_t*>(row + y / 2 * K_ATOM + (((y % 2) * 4 + n) ^ g) * 16) = as_u32(__hmul2(as_h2(z[n]), d));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(&full[slot]);
             next();
-            if (i + 1 < tiles) {
-                find(i + 1);
-                load_k();
-            }
-            good = mbar_wait(&empty[slot], phase, failed);
-            if (!good) break;
-            to = ring + slot * SLOT;
+            // rows behind the last hold anything
+            const long long left = si.len - (i * TK + gt * 16 + 8 * h + 2 * c);
+            if (left < 2)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint8_t* row = to + g * 128 + ((dw * 2 + h) ^ g) * 16 + 4 * c;   // 16 bytes: 8 tokens
+                for (int y = 0; y < NB; y++) cur.vs[y] &= left == 1 ? 0xffffu : 0u;
+            if (!mbar_wait(&empty[slot], phase, failed)) break;
+            row = ring + slot * SLOT + g * 128 + ((gt * 2 + h) ^ g) * 16 + 4 * c;   // 16 bytes: 8 tokens
 #pragma unroll
-                for (int y = 0; y < NB; y++) {
-                    const __half2 d = __hmul2(as_h2(vs[h][y]), vmul);
-                    uint32_t z[4];
-                    codes(z, vw[h][y]);
+            for (int y = 0; y < NB; y++) {
+                const __half2 d = __hmul2(as_h2(cur.vs[y]), vmul);
+                uint32_t z[4];
+                codes(z, cur.vw[y]);
 #pragma unroll
-                    for (int n = 0; n < 4; n++)
-                        *reinterpret_cast<uint32_t*>(row + (32 * y + 8 * n) * 128) = as_u32(__hmul2(as_h2(z[n]), d));
-                }
+                for (int n = 0; n < 4; n++)
+                    *reinterpret_cast<uint32_t*>(row + (32 * y + 8 * n) * 128) = as_u32(__hmul2(as_h2(z[n]), d));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(&full[slot]);
             next();
+            cur = nxt;
         }
-    } else if (tiles) {
-        // ================================ the MMAs
-        constexpr uint32_t IDESC_S = (1u << 4) | ((TK >> 3) << 17) | ((QT >> 4) << 24);
-        constexpr uint32_t IDESC_O = (1u << 4) | ((HD >> 3) << 17) | ((QT >> 4) << 24);
-        const uint64_t dq = sw128_desc(saddr(s_q)), dr = sw128_desc(saddr(ring));
-        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        // the warp is in step throughout; one lane issues
-        auto scores = [&](int q, int i, int slot, bool last) {
-            const uint32_t d = tm + q * 128 + (i & 1) * TK;
-            const uint64_t x = dq + (q * Q_BYTES >> 4), y = dr + (slot * SLOT >> 4);
-            if (elect_one()) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == SW + DW && tiles) {
+            // ================================ the MMAs
+            constexpr uint32_t IDESC_S = (1u << 4) | ((TK >> 3) << 17) | ((QT >> 4) << 24);
+            constexpr uint32_t IDESC_O = (1u << 4) | ((HD >> 3) << 17) | ((QT >> 4) << 24);
+            const uint64_t dq = sw128_desc(saddr(s_q)), dr = sw128_desc(saddr(ring));
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            // the warp is in step throughout; one lane issues
+            auto scores = [&](int q, int i, int slot, bool last) {
+                const uint32_t d = tm + q * 128 + (i & 1) * TK;
+                const uint64_t x = dq + (q * Q_BYTES >> 4), y = dr + (slot * SLOT >> 4);
+                if (elect_one()) {
 #pragma unroll
-                for (int s = 0; s < 2 * NB; s++)
-                    mma_f16_ss(d, x + ((s / 4 * ATOM + s % 4 * 32) >> 4), y + ((s / 4 * K_ATOM + s % 4 * 32) >> 4), IDESC_S, s > 0);
-                commit(&s_full[q][i & 1]);
-                if (last) commit(&empty[slot]);
-            }
-            __syncwarp();
-        };
-        auto values = [&](int q, int i, int slot, bool last) {
-            const uint32_t d = tm + 256 + q * 128, x = tm + q * 128 + (i & 1) * TK;
-            const uint64_t y = dr + (slot * SLOT >> 4);
-            if (elect_one()) {
-#pragma unroll
-                for (int s = 0; s < TK / 16; s++) mma_f16_ts(d, x + 8 * s, y + (s * 32 >> 4), IDESC_O, i > 0 || s > 0);
-                commit(&pv_done[q]);
-                if (last) commit(&empty[slot]);
-            }
-            __syncwarp();
-        };
-        auto fence = [] { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); };
-        int kslot = 0, vslot = 1;                // of K of the next tile, and V of this one
-        uint32_t kphase = 0, vphase = 0;
-        auto step = [](int& slot, uint32_t& phase) {
-            slot += 2;
-            if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
-        };
-        auto wait = [&](uint64_t* m, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(m, parity, failed)); };
-        bool good = wait(&q_full, 0) && wait(&full[0], 0);
-        if (good) {
-            fence();
-            scores(0, 0, 0, false);
-            scores(1, 0, 0, true);
-            step(kslot, kphase);
-        }
-        for (int i = 0; i < tiles && good; i++) {
-            const bool more = i + 1 < tiles;
-            if (more) good = wait(&full[kslot], kphase);
-            for (int q = 0; q < 2 && good; q++) {
-                if (more) {   // the next scores go into the other half of S, which O's last sum has read
-                    fence();
-                    scores(q, i + 1, kslot, q == 1);
+                    for (int s = 0; s < 2 * NB; s++)
+                        mma_f16_ss(d, x + ((s / 4 * ATOM + s % 4 * 32) >> 4), y + ((s / 4 * K_ATOM + s % 4 * 32) >> 4), IDESC_S, s > 0);
+                    commit(&s_full[q][i & 1]);
+                    if (last) commit(&empty[slot]);
                 }
-                good = (q || wait(&full[vslot], vphase)) && wait(&p_ready[q][i & 1], i >> 1 & 1);
-                if (!good) break;
+                __syncwarp();
+            };
+            auto values = [&](int q, int i, int slot, bool last) {
+                const uint32_t d = tm + 256 + q * 128, x = tm + q * 128 + (i & 1) * TK;
+                const uint64_t y = dr + (slot * SLOT >> 4);
+                if (elect_one()) {
+#pragma unroll
+                    for (int s = 0; s < TK / 16; s++) mma_f16_ts(d, x + 8 * s, y + (s * 32 >> 4), IDESC_O, i > 0 || s > 0);
+                    commit(&pv_done[q]);
+                    if (last) commit(&empty[slot]);
+                }
+                __syncwarp();
+            };
+            auto fence = [] { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); };
+            int kslot = 0, vslot = 1;                // of K of the next tile, and V of this one
+            uint32_t kphase = 0, vphase = 0;
+            auto step = [](int& slot, uint32_t& phase) {
+                slot += 2;
+                if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
+            };
+            auto wait = [&](uint64_t* m, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(m, parity, failed)); };
+            bool good = wait(&q_full, 0) && wait(&full[0], 0);
+            if (good) {
                 fence();
-                values(q, i, vslot, q == 1);
+                scores(0, 0, 0, false);
+                scores(1, 0, 0, true);
+                step(kslot, kphase);
             }
-            step(kslot, kphase);
-            step(vslot, vphase);
-        }
-        if (!good) {   // what is under way ends before the TMEM is freed: one more commit behind it all
-            if (elect_one()) commit(&q_full);
-            const long long t0 = clock64();
-            while (!mbar_try(&q_full, 1) && clock64() - t0 < WAIT_CYCLES / 16) {
+            for (int i = 0; i < tiles && good; i++) {
+                const bool more = i + 1 < tiles;
+                if (more) good = wait(&full[kslot], kphase);
+                for (int q = 0; q < 2 && good; q++) {
+                    if (more) {   // the next scores go into the other half of S, which O's last sum has read
+                        fence();
+                        scores(q, i + 1, kslot, q == 1);
+                    }
+                    good = (q || wait(&full[vslot], vphase)) && wait(&p_ready[q][i & 1], i >> 1 & 1);
+                    if (!good) break;
+                    fence();
+                    values(q, i, vslot, q == 1);
+                }
+                step(kslot, kphase);
+                step(vslot, vphase);
+            }
+            if (!good) {   // what is under way ends before the TMEM is freed: one more commit behind it all
+                if (elect_one()) commit(&q_full);
+                const long long t0 = clock64();
+                while (!mbar_try(&q_full, 1) && clock64() - t0 < WAIT_CYCLES / 16) {
+                }
             }
         }
     }
@@ -477,13 +530,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
 
 size_t r256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// Items that T tokens of B sequences have at most.
+long long item_cap(const KvqBatch& b, int T, int R) { return (long long)T * R / (2 * QT) + b.B; }
+
 template <int DT, int NB>
 cudaError_t launch_tc(const TcArgs& t, cudaStream_t s) {
     constexpr int smem = 2 * (NB / 2) * QT * 128 + SLOTS * 4096 * NB + 1024;
     cudaError_t e = cudaFuncSetAttribute(k_kvq_tc<DT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    const long long rows = (long long)t.a.b.max_new * t.a.R;
-    k_kvq_tc<DT, NB><<<dim3((unsigned)((rows + 2 * QT - 1) / (2 * QT)), t.a.c.nkv, t.a.b.B), THREADS, smem, s>>>(t);
+    k_kvq_tc<DT, NB><<<(unsigned)(item_cap(t.a.b, t.a.T, t.a.R) * t.a.c.nkv), THREADS, smem, s>>>(t);
     return cudaGetLastError();
 }
 
@@ -491,22 +546,32 @@ cudaError_t launch_tc(const TcArgs& t, cudaStream_t s) {
 
 // Where a tile of 256 rows is mostly full, and there are CTAs for about half of the SMs: few
 // tiles over a long cache are cut along the cache by the other kernel.
-bool attn_tc_takes(int dtype, const KvqCache& c, const KvqBatch& b, int R) {
+bool attn_tc_takes(int dtype, const KvqCache& c, const KvqBatch& b, int T, int R) {
     const long long rows = (long long)b.max_new * R, items = (rows + 2 * QT - 1) / (2 * QT) * c.nkv * b.B;
-    return dtype != TGX_F32 && (c.hd == 64 || c.hd == 128) && rows >= QT && items >= 64 && c.nkv <= 65535 && b.B <= 65535;
+    return dtype != TGX_F32 && (c.hd == 64 || c.hd == 128) && rows >= QT && items >= 64 && c.nkv <= 65535 && b.B <= 65535 &&
+           item_cap(b, T, R) * c.nkv <= 0x7fffffff;
 }
 
-size_t attn_tc_scratch(const KvqCache& c, const KvqBatch& b) {
-    return r256((size_t)c.nkv * b.B * 4) + r256((size_t)c.nkv * b.B * 8);
+size_t attn_tc_scratch(const KvqCache& c, const KvqBatch& b, int T, int R) {
+    return r256((size_t)c.nkv * b.B * 4) + r256((size_t)c.nkv * b.B * 8) + r256((size_t)item_cap(b, T, R) * 8) + 256;
 }
 
 cudaError_t launch_attn_tc(int dtype, const AttnKvqArgs& a, void* scratch, const int** only, cudaStream_t s) {
-    int* marks = reinterpret_cast<int*>(scratch);
-    int2* exps = reinterpret_cast<int2*>((uint8_t*)scratch + r256((size_t)a.c.nkv * a.b.B * 4));
-    k_kvq_scan<<<dim3(a.c.nkv, a.b.B), 512, 0, s>>>(a, marks, exps);
+    uint8_t* at = (uint8_t*)scratch;
+    auto take = [&](size_t n) {
+        void* p = at;
+        at += r256(n);
+        return p;
+    };
+    const int cap = (int)item_cap(a.b, a.T, a.R);
+    int* marks = (int*)take((size_t)a.c.nkv * a.b.B * 4);
+    int2* exps = (int2*)take((size_t)a.c.nkv * a.b.B * 8);
+    int2* order = (int2*)take((size_t)cap * 8);
+    int* items = (int*)take(4);
+    k_kvq_scan<<<dim3(a.c.nkv, a.b.B), 1024, 0, s>>>(a, marks, exps, order, items, cap);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    const TcArgs t{a, marks, exps};
+    const TcArgs t{a, marks, exps, order, items};
     *only = marks;   // `only` may be a's own
     if (dtype == TGX_BF16) return a.c.hd == 128 ? launch_tc<TGX_BF16, 4>(t, s) : launch_tc<TGX_BF16, 2>(t, s);
     return a.c.hd == 128 ? launch_tc<TGX_F16, 4>(t, s) : launch_tc<TGX_F16, 2>(t, s);
