@@ -7,13 +7,19 @@
 //   p = 2^(s - m) a thread per query row, reading its TMEM lane; P goes back over S as fp16
 //   O += P V      A from TMEM, B the transposed V tile
 // Codes are turned into fp16 values once per CTA and tile, code * d rounded to 11 bits, by eight
-// warps that read the granules straight into registers (the next tile's while this one's are
-// converted) and write the 128-byte-swizzled operands; a ring of six slots holds K, V, K, ...
-// The layout of the cache makes both K-major operands of 4-byte pieces that 32 lanes store
-// without a bank conflict: two dimensions of a token for K, two tokens of a dimension for V.
-// The scores of a tile are issued before the softmax of the one in front is waited for, so the
-// softmax warps go from tile to tile (with one S per query tile and tiles of 128 tokens they
-// waited: 254 us instead of TCUS for three prompts of up to 1500 tokens behind up to 2500).
+// warps, four for K and four for V, that read the granules straight into registers (the next
+// tile's while this one's are converted) and write the 128-byte-swizzled operands; a ring of six
+// slots holds K, V, K, ...  The layout of the cache makes both K-major operands of 4-byte pieces
+// that 32 lanes store without a bank conflict: two dimensions of a token for K, two tokens of a
+// dimension for V.  The scores of a tile are issued before the softmax of the one in front is
+// waited for, so the softmax warps go from tile to tile.
+//
+// Three prompts of up to 1500 tokens behind up to 2500 (32 heads over 4 kv heads of 128): 156 us,
+// 1.1 us a pair of tiles of 64 tokens.  There the issue of the MMAs takes 1700 of 2350 cycles (24
+// of them, 70 cycles each; at N = 64 the tensor cores' own time is 1024), the softmax 1300.
+// 254 us with tiles of 128 tokens and one S per query tile; 246 with four conversion warps,
+// query rows read and written a row a thread (34000 cycles before the first tile, 9000 now), and
+// the items of a sequence next to one another instead of in order of the rows they see.
 //
 // m moves, and O in TMEM is rescaled, only when a row's scores leave 2^SLACK of it.  q rows, K
 // and V are held in fp16 times powers of two: q's largest in 2^13 .. 2^14, the largest scale of
@@ -30,7 +36,7 @@ namespace tg {
 namespace {
 
 constexpr int QT = 128;          // query rows of a tile
-constexpr int TK = 64;           // tokens of a tile: half a granule per conversion warp
+constexpr int TK = 64;           // tokens of a tile: K or V of a granule per conversion warp
 constexpr int SLOTS = 6;
 constexpr int SW = 8, DW = 8;    // softmax and conversion warps; one more for the MMAs
 constexpr int THREADS = 32 * (SW + DW + 4);
@@ -55,8 +61,29 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
             d),
         "r"(a), "l"(b), "r"(idesc), "r"(add));
 }
-__device__ __forceinline__ void commit(uint64_t* m) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(m)) : "memory");
+__device__ __forceinline__ void commit(uint32_t m) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(m) : "memory");
+}
+// Two fp32 numbers an instruction.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t z;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(z) : "f"(x), "f"(y));
+    return z;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t x) {
+    float2 z;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(z.x), "=f"(z.y) : "l"(x));
+    return z;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t z;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(z) : "l"(a), "l"(b), "l"(c));
+    return z;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t z;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(z) : "l"(a), "l"(b));
+    return z;
 }
 // The exponent by which a row of q is divided, from its largest magnitude.
 __device__ __forceinline__ int q_exp(unsigned top) {
@@ -171,12 +198,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     constexpr int HD = 32 * NB, ATOM = QT * 128;               // bytes of 64 dimensions of 128 rows
     constexpr int Q_BYTES = NB / 2 * ATOM, SLOT = 4096 * NB, K_ATOM = TK * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t q_full, full[SLOTS], empty[SLOTS], s_full[2][2], p_ready[2][2], pv_done[2];
+    __shared__ __align__(8) uint64_t s_bars[11 + 2 * SLOTS];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
     __shared__ __align__(4) uint8_t s_valid[8][TK / 16];   // [tile % 8]: whether its granules exist
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t bars = saddr_kept(s_bars), q_full = bars;
+    auto pv_done = [&](int q) { return bars + 8 + 8 * q; };
+    auto s_full = [&](int q, int i) { return bars + 24 + 16 * q + 8 * (i & 1); };    // of tile i
+    auto p_ready = [&](int q, int i) { return bars + 56 + 16 * q + 8 * (i & 1); };
+    auto full = [&](int slot) { return bars + 88 + 8 * slot; };
+    auto empty = [&](int slot) { return bars + 88 + 8 * SLOTS + 8 * slot; };
 
     const int item = blockIdx.x / a.c.nkv, j = blockIdx.x % a.c.nkv;   // the longest first
     if (item >= *t.items) return;
@@ -192,12 +225,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     uint8_t* const ring = sm + 2 * Q_BYTES;
 
     if (tid == 0) {
-        mbar_init(&q_full, 32 * SW);
-        for (int i = 0; i < SLOTS; i++) mbar_init(&full[i], 32 * DW), mbar_init(&empty[i], 1);
-        for (int i = 0; i < 2; i++) {
-            for (int x = 0; x < 2; x++) mbar_init(&s_full[i][x], 1), mbar_init(&p_ready[i][x], QT);
-            mbar_init(&pv_done[i], 1);
-        }
+        mbar_init(&s_bars[0], 32 * SW);
+        for (int i = 1; i < 7; i++) mbar_init(&s_bars[i], 1);
+        for (int i = 7; i < 11; i++) mbar_init(&s_bars[i], QT);
+        for (int i = 0; i < SLOTS; i++) mbar_init(&s_bars[11 + i], 16 * DW), mbar_init(&s_bars[11 + SLOTS + i], 1);
         s_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;");
     }
@@ -211,9 +242,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     const uint32_t tmem = s_tmem;   // S (and P) of query tile q at 128 q + 64 (tile & 1), O at 256 + 128 q
     volatile int* failed = &s_failed;
 
-    // 640 threads start with 96 registers each (61440): 256 x 128 + 256 x 80 + 128 x 64 are as many
+    // 640 threads start with 96 registers each (61440): 256 x 120 + 256 x 80 + 128 x 72 are 60416
     if (warp < SW) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
         // ================================ a thread per query row
         const int q = warp >> 2, r = (warp & 3) * 32 + lane, x0 = q * QT;
         const bool ok = x0 + r < nrows;
@@ -266,14 +297,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             const int e = q_exp(top), half = e / 2;
             fac = a.scale * pow2(half) * pow2(e - half) * pow2(ex.x);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&q_full);
+            mbar_arrive(q_full);
         }
         const uint32_t s_at = tmem + q * 128 + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t o_at = tmem + 256 + q * 128 + ((uint32_t)((warp & 3) * 32) << 16);
         float m = -INFINITY, off = 0.0f, l = 0.0f;
         bool good = true;
         for (int i = 0; i < tiles && good; i++) {
-            good = __all_sync(0xffffffffu, mbar_wait(&s_full[q][i & 1], i >> 1 & 1, failed));
+            good = __all_sync(0xffffffffu, mbar_wait(s_full(q, i), i >> 1 & 1, failed));
             if (!good) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t have = *reinterpret_cast<const volatile uint32_t*>(s_valid[i & 7]), s_i = s_at + (i & 1) * TK;
@@ -284,6 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             const bool edge = t0 + TK > lim_min || have != 0x01010101u;
             if (edge) {
+                asm volatile("");   // a branch: 64 predicated compares cost every tile otherwise
 #pragma unroll
                 for (int x = 0; x < TK; x++)   // hidden from the row, or not in the cache
                     if (t0 + x >= lim || !(have >> (x / 16 * 8) & 1)) v[x / 32][x % 32] = __float_as_uint(-INFINITY);
@@ -298,7 +330,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
                 off = m == -INFINITY ? 0.0f : P_EXP - m;
                 l *= f;
                 if (i) {
-                    good = __all_sync(0xffffffffu, mbar_wait(&pv_done[q], (i - 1) & 1, failed));   // O is at rest
+                    good = __all_sync(0xffffffffu, mbar_wait(pv_done(q), (i - 1) & 1, failed));   // O is at rest
                     if (!good) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -313,25 +345,25 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
                 }
             }
             uint32_t p[32];
-            float sum[2] = {0.0f, 0.0f};
+            uint64_t sum = 0;   // fp32 sums of the even and odd columns
+            const uint64_t fac2 = pack2(fac, fac), off2 = pack2(off, off);
 #pragma unroll
             for (int x = 0; x < 32; x++) {
-                float y[2];
-#pragma unroll
-                for (int z = 0; z < 2; z++) {
-                    const float s = __uint_as_float(v[x / 16][2 * (x % 16) + z]);
-                    y[z] = ex2(fmaf(s, fac, off));
-                    sum[z] += y[z];
-                }
-                p[x] = as_u32(__floats2half2_rn(y[0], y[1]));
+                const float2 s = unpack2(fma2(pack2(__uint_as_float(v[x / 16][2 * (x % 16)]), __uint_as_float(v[x / 16][2 * (x % 16) + 1])), fac2, off2));
+                const float y0 = ex2(s.x), y1 = ex2(s.y);
+                sum = add2(sum, pack2(y0, y1));
+                p[x] = as_u32(__floats2half2_rn(y0, y1));
             }
-            l += sum[0] + sum[1];
+            l += unpack2(sum).x + unpack2(sum).y;
             tmem_st(s_i, p);   // over scores that have been read
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            mbar_arrive(&p_ready[q][i & 1]);
+            mbar_arrive(p_ready(q, i));
         }
-        if (good && tiles) good = __all_sync(0xffffffffu, mbar_wait(&pv_done[q], (tiles - 1) & 1, failed));
+        // The sums of the last two tiles, one by one: this warp's scores may have come before another
+        // warp's p of the tile in front, and a parity tells neighbouring phases apart, no more.
+        for (int i = max(0, tiles - 2); i < tiles && good; i++)
+            good = __all_sync(0xffffffffu, mbar_wait(pv_done(q), i & 1, failed));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inv = !good ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
         const float v2 = pow2(ex.y);
@@ -365,94 +397,104 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     } else if (warp < SW + DW) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        // ================================ codes into operands: half a granule of each tile per warp
-        const int dw = warp - SW, gt = dw >> 1, h = dw & 1, g = lane >> 2, c = lane & 3, gpp = a.c.pt >> 4;
-        const __half2 kmul = __float2half2_rn(pow2(-ex.x)), vmul = __float2half2_rn(pow2(-ex.y));
+        // ================================ codes into operands: K's or V's of a granule per warp and tile
+        const int dw = warp - SW, gt = dw & 3, g = lane >> 2, c = lane & 3, gpp = a.c.pt >> 4;
+        const bool is_v = dw >= DW / 2;
+        const __half2 mul = __float2half2_rn(pow2(is_v ? -ex.y : -ex.x));
         const uint32_t k1024 = a.k1024;
         struct Raw {
-            uint32_t kw[NB], ks[NB / 2], vw[NB], vs[NB];
+            uint32_t w[2][NB], s[2][NB];   // of the granule's two halves: codes, and scales (K's: half as many)
             bool there;
+        } cur, nxt;
+        // the page table's entry and the granule of its page of the next tile's granule; the page is read a tile ahead
+        const int* entry = a.b.table + (size_t)b * a.b.max_pages + gt / gpp;
+        int gp = gt % gpp, ahead = gp, page = 0, tok = gt * 16;
+        auto read_page = [&](int t) {
+            while (ahead >= gpp) ahead -= gpp, entry++;
+            page = t < seen ? *entry : 0;   // what lies behind the last row that is seen, the rows' limits hide
         };
-        auto page_of = [&](int i) -> int {   // the page of tile i's granule; 0 behind the last row that is seen
-            const int gi = i * (TK / 16) + gt;
-            return gi * 16 < seen ? a.b.table[(size_t)b * a.b.max_pages + gi / gpp] : 0;
-        };
-        auto load = [&](Raw& x, int i, int page) {
-            const int gi = i * (TK / 16) + gt;
-            const bool in = gi * 16 < seen;   // what is not, the rows' limits hide
+        auto load = [&](Raw& x) {
+            const bool in = tok < seen;
             x.there = !in || (page >= 0 && page < a.c.n_pages);
             if (!x.there && lane == 0) kvq_flag(a.b, TGX_KVQ_BAD_PAGE);
 #pragma unroll
-            for (int y = 0; y < NB; y++) x.kw[y] = x.vw[y] = x.vs[y] = 0;
-#pragma unroll
-            for (int y = 0; y < NB / 2; y++) x.ks[y] = 0;
+            for (int y = 0; y < 2 * NB; y++) x.w[y / NB][y % NB] = x.s[y / NB][y % NB] = 0;
             if (in && x.there) {
-                const uint8_t* at = kvq_granule(a.c, page, j, gi % gpp * 16);
-                load_words<NB>(x.kw, at + (h * 32 + lane) * NB * 4);
-                load_words<NB / 2>(x.ks, at + 16 * HD + (h * 8 + g) * NB * 2);
-                load_words<NB>(x.vw, at + 8 * HD + (h * 32 + lane) * NB * 4);
-                load_words<NB>(x.vs, at + 17 * HD + (h * 4 + c) * NB * 4);
+                const uint8_t* at = kvq_granule(a.c, page, j, gp * 16);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (is_v) {
+                        load_words<NB>(x.w[h], at + 8 * HD + (h * 32 + lane) * NB * 4);
+                        load_words<NB>(x.s[h], at + 17 * HD + (h * 4 + c) * NB * 4);
+                    } else {
+                        load_words<NB>(x.w[h], at + (h * 32 + lane) * NB * 4);
+                        uint32_t (&half)[NB / 2] = reinterpret_cast<uint32_t (&)[NB / 2]>(x.s[h]);
+                        load_words<NB / 2>(half, at + 16 * HD + (h * 8 + g) * NB * 2);
+                    }
+                }
             }
+            gp += TK / 16, ahead = gp;
+            tok += TK;
+            read_page(tok);
+            gp = ahead;
         };
-        int slot = 0;
+        int slot = is_v;
         uint32_t phase = 1;   // of `empty`: a fresh barrier's wait for it passes
-        auto next = [&] {
-            if (++slot == SLOTS) slot = 0, phase ^= 1;
-        };
         // the lane's four code pairs of a word
         auto codes = [&](uint32_t (&z)[4], uint32_t w) {
             const uint32_t x = w >> 8;
             z[0] = codes_lo<false>(w, k1024), z[1] = codes_hi<false>(w, k1024);
             z[2] = codes_lo<false>(x, k1024), z[3] = codes_hi<false>(x, k1024);
         };
-        Raw cur, nxt;
-        int page = 0;   // of the next tile
-        if (tiles) {
-            load(cur, 0, page_of(0));
-            page = page_of(1);
-        }
+        read_page(tok);
+        load(cur);
+#pragma unroll 2
         for (int i = 0; i < tiles; i++) {
-            load(nxt, i + 1, page);
-            page = page_of(i + 2);
-            if (lane == 0 && h == 0) s_valid[i & 7][gt] = cur.there ? 1 : 0;
-            if (!mbar_wait(&empty[slot], phase, failed)) break;
-            uint8_t* row = ring + slot * SLOT + (gt * 16 + 8 * h + g) * 128 + 4 * c;
+            load(nxt);
+            if (lane == 0 && !is_v) s_valid[i & 7][gt] = cur.there ? 1 : 0;
+            if (!mbar_wait(empty(slot), phase, failed)) break;
+            if (!is_v) {
+                uint8_t* row = ring + slot * SLOT + (gt * 16 + g) * 128 + 4 * c;
 #pragma unroll
-            for (int y = 0; y < NB; y++) {
-                const __half2 pair = as_h2(cur.ks[y / 2]);
-                const __half2 d = __hmul2(y & 1 ? __high2half2(pair) : __low2half2(pair), kmul);
-                uint32_t z[4];
-                codes(z, cur.kw[y]);
+                for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int n = 0; n < 4; n++)
-                    *reinterpret_cast<uint32_t*>(row + y / 2 * K_ATOM + (((y % 2) * 4 + n) ^ g) * 16) = as_u32(__hmul2(as_h2(z[n]), d));
+                    for (int y = 0; y < NB; y++) {
+                        const __half2 pair = as_h2(cur.s[h][y / 2]);
+                        const __half2 d = __hmul2(y & 1 ? __high2half2(pair) : __low2half2(pair), mul);
+                        uint32_t z[4];
+                        codes(z, cur.w[h][y]);
+#pragma unroll
+                        for (int n = 0; n < 4; n++)
+                            *reinterpret_cast<uint32_t*>(row + h * 1024 + y / 2 * K_ATOM + (((y % 2) * 4 + n) ^ g) * 16) = as_u32(__hmul2(as_h2(z[n]), d));
+                    }
+            } else {
+                const long long left = si.len - (i * TK + gt * 16);   // rows behind the last hold anything
+                if (left < 16)
+#pragma unroll
+                    for (int y = 0; y < 2 * NB; y++) {
+                        const int t = y / NB * 8 + 2 * c;
+                        if (t + 1 >= left) cur.s[y / NB][y % NB] &= t < left ? 0xffffu : 0u;
+                    }
+                uint8_t* row = ring + slot * SLOT + g * 128 + 4 * c;   // 16 bytes: 8 tokens
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int y = 0; y < NB; y++) {
+                        const __half2 d = __hmul2(as_h2(cur.s[h][y]), mul);
+                        uint32_t z[4];
+                        codes(z, cur.w[h][y]);
+#pragma unroll
+                        for (int n = 0; n < 4; n++)
+                            *reinterpret_cast<uint32_t*>(row + ((gt * 2 + h) ^ g) * 16 + (32 * y + 8 * n) * 128) = as_u32(__hmul2(as_h2(z[n]), d));
+                    }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&full[slot]);
-            next();
-            // rows behind the last hold anything
-            const long long left = si.len - (i * TK + gt * 16 + 8 * h + 2 * c);
-            if (left < 2)
-#pragma unroll
-                for (int y = 0; y < NB; y++) cur.vs[y] &= left == 1 ? 0xffffu : 0u;
-            if (!mbar_wait(&empty[slot], phase, failed)) break;
-            row = ring + slot * SLOT + g * 128 + ((gt * 2 + h) ^ g) * 16 + 4 * c;   // 16 bytes: 8 tokens
-#pragma unroll
-            for (int y = 0; y < NB; y++) {
-                const __half2 d = __hmul2(as_h2(cur.vs[y]), vmul);
-                uint32_t z[4];
-                codes(z, cur.vw[y]);
-#pragma unroll
-                for (int n = 0; n < 4; n++)
-                    *reinterpret_cast<uint32_t*>(row + (32 * y + 8 * n) * 128) = as_u32(__hmul2(as_h2(z[n]), d));
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&full[slot]);
-            next();
+            mbar_arrive(full(slot));
+            if ((slot += 2) >= SLOTS) slot -= SLOTS, phase ^= 1;
             cur = nxt;
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == SW + DW && tiles) {
             // ================================ the MMAs
             constexpr uint32_t IDESC_S = (1u << 4) | ((TK >> 3) << 17) | ((QT >> 4) << 24);
@@ -467,8 +509,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
 #pragma unroll
                     for (int s = 0; s < 2 * NB; s++)
                         mma_f16_ss(d, x + ((s / 4 * ATOM + s % 4 * 32) >> 4), y + ((s / 4 * K_ATOM + s % 4 * 32) >> 4), IDESC_S, s > 0);
-                    commit(&s_full[q][i & 1]);
-                    if (last) commit(&empty[slot]);
+                    commit(s_full(q, i));
+                    if (last) commit(empty(slot));
                 }
                 __syncwarp();
             };
@@ -478,8 +520,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
                 if (elect_one()) {
 #pragma unroll
                     for (int s = 0; s < TK / 16; s++) mma_f16_ts(d, x + 8 * s, y + (s * 32 >> 4), IDESC_O, i > 0 || s > 0);
-                    commit(&pv_done[q]);
-                    if (last) commit(&empty[slot]);
+                    commit(pv_done(q));
+                    if (last) commit(empty(slot));
                 }
                 __syncwarp();
             };
@@ -490,8 +532,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
                 slot += 2;
                 if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
             };
-            auto wait = [&](uint64_t* m, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(m, parity, failed)); };
-            bool good = wait(&q_full, 0) && wait(&full[0], 0);
+            auto wait = [&](uint32_t m, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(m, parity, failed)); };
+            bool good = wait(q_full, 0) && wait(full(0), 0);
             if (good) {
                 fence();
                 scores(0, 0, 0, false);
@@ -500,13 +542,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             }
             for (int i = 0; i < tiles && good; i++) {
                 const bool more = i + 1 < tiles;
-                if (more) good = wait(&full[kslot], kphase);
+                if (more) good = wait(full(kslot), kphase);
                 for (int q = 0; q < 2 && good; q++) {
                     if (more) {   // the next scores go into the other half of S, which O's last sum has read
                         fence();
                         scores(q, i + 1, kslot, q == 1);
                     }
-                    good = (q || wait(&full[vslot], vphase)) && wait(&p_ready[q][i & 1], i >> 1 & 1);
+                    good = (q || wait(full(vslot), vphase)) && wait(p_ready(q, i), i >> 1 & 1);
                     if (!good) break;
                     fence();
                     values(q, i, vslot, q == 1);
@@ -515,9 +557,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
                 step(vslot, vphase);
             }
             if (!good) {   // what is under way ends before the TMEM is freed: one more commit behind it all
-                if (elect_one()) commit(&q_full);
+                if (elect_one()) commit(q_full);
                 const long long t0 = clock64();
-                while (!mbar_try(&q_full, 1) && clock64() - t0 < WAIT_CYCLES / 16) {
+                while (!mbar_try(q_full, 1) && clock64() - t0 < WAIT_CYCLES / 16) {
                 }
             }
         }

@@ -9,26 +9,34 @@ constexpr long long WAIT_CYCLES = 2000000000ll;   // about a second
 
 __device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// A shared address kept in a register: otherwise every use forms it anew, from a special register
+// that takes its time.
+__device__ __forceinline__ uint32_t saddr_kept(const void* p) {
+    uint32_t x;
+    asm volatile("mov.u32 %0, %1;" : "=r"(x) : "r"(saddr(p)));
+    return x;
+}
+
 __device__ __forceinline__ void mbar_init(uint64_t* m, int n) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(saddr(m)), "r"(n));
 }
 __device__ __forceinline__ void mbar_expect(uint64_t* m, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(saddr(m)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint64_t* m) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(saddr(m)) : "memory");
+__device__ __forceinline__ void mbar_arrive(uint32_t m) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(m) : "memory");
 }
-__device__ __forceinline__ bool mbar_try(uint64_t* m, uint32_t parity) {
+__device__ __forceinline__ bool mbar_try(uint32_t m, uint32_t parity) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done)
-        : "r"(saddr(m)), "r"(parity)
+        : "r"(m), "r"(parity)
         : "memory");
     return done;
 }
 // Waits for the phase; false once the limit is over here or a wait has failed elsewhere in the CTA.
-__device__ __forceinline__ bool mbar_wait(uint64_t* m, uint32_t parity, volatile int* failed) {
+__device__ __forceinline__ bool mbar_wait(uint32_t m, uint32_t parity, volatile int* failed) {
     if (mbar_try(m, parity)) return true;
     const long long t0 = clock64();
     while (!mbar_try(m, parity)) {
@@ -39,6 +47,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* m, uint32_t parity, volatile
         }
     }
     return true;
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* m) { mbar_arrive(saddr(m)); }
+__device__ __forceinline__ bool mbar_try(uint64_t* m, uint32_t parity) { return mbar_try(saddr(m), parity); }
+__device__ __forceinline__ bool mbar_wait(uint64_t* m, uint32_t parity, volatile int* failed) {
+    return mbar_wait(saddr(m), parity, failed);
 }
 // The same for what must land before the CTA may end.
 __device__ __forceinline__ void mbar_drain(uint64_t* m, uint32_t parity) {
