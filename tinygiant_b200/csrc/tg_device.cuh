@@ -191,7 +191,7 @@ __device__ __forceinline__ void topk_softmax_block(const float* sl, int E, int k
         int rank = 0;
         for (int j = 0; j < E; j++) {
             float lj = sl[j];
-            rank += (lj > li) || (lj == li && j > i);
+            rank += (lj > li) || (!(li > lj) && j > i);   // NaN too has its place: every sidx is written
         }
         if (rank < k) sidx[k - 1 - rank] = i;
     }
