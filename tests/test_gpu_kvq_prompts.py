@@ -1,0 +1,208 @@
+"""Attention over the paged 4-bit cache for many query rows of 16-bit types (tcgen05): head counts
+whose rows cut tiles anywhere, partial pages and tiles, scales that are not finite, values out of
+the ordinary, and the batch's faults."""
+from __future__ import annotations
+
+import pytest
+
+from tests import serve_ref as R
+from tests.test_gpu_kvq import BF16, F16, Setup, close
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+# several sequences each, so that there are tiles enough for the SMs
+MANY = [(140, 300), (257, 257), (1, 90), (33, 900), (0, 40), (200, 201), (16, 2), (64, 1000)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("nh,nkv,hd,page", [(12, 4, 64, 48), (28, 4, 128, 16), (32, 1, 128, 1024), (8, 8, 128, 64),
+                                            (160, 5, 64, 16), (10, 2, 128, 128)])
+def test_heads_and_pages(nh, nkv, hd, page, dtype):
+    s = Setup(MANY * (1 if nkv * nh > 60 else 2), nh, nkv, hd, page, dtype, seed=nh + page)
+    close(s.cache.attention(s.batch, s.q), *s.expect(), hd, 1000, dtype)
+    s.batch.check()
+
+
+@pytest.mark.parametrize("n,r", [(128, 128), (256, 256), (32, 2048), (32, 2049), (33, 2111), (512, 513), (480, 3000)])
+def test_even_tiles(n, r):
+    """Rows and lengths at, before and behind the tiles' edges, alike in all sequences."""
+    s = Setup([(n, r)] * 8, 32, 8, 64, 32, BF16, seed=n)
+    close(s.cache.attention(s.batch, s.q), *s.expect(), 64, r, BF16)
+
+
+def test_long_context():
+    s = Setup([(300, 20011), (40, 9000), (500, 500)], 32, 4, 128, 64, BF16, seed=3)
+    close(s.cache.attention(s.batch, s.q), *s.expect(), 128, 20011, BF16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("values", [1e-6, 1e-3, 300.0])
+def test_value_ranges(dtype, values):
+    """V far from 1 (fp16 blocks that are nearly or wholly zero among them), scores far apart and
+    all equal, q near its type's smallest and beyond what products in fp16 could hold."""
+    s = Setup([(200, 700)] * 6, 16, 2, 128, 64, dtype, values=values, seed=9)
+    s.q[0::5] *= 20
+    s.q[1::5] = 0
+    s.q[2::5] *= 1e-4
+    s.q[3] = 3e4
+    s.q[3, :, 1::2] = -3e4
+    out = s.cache.attention(s.batch, s.q)
+    ref = s.expect()
+    keep = [t for t in range(s.T) if t != 3]   # one key takes all of row 3: finite is what is asked of it
+    got, ref = out[keep], [x[keep] for x in ref]
+    if dtype == F16:
+        # Below 2^-14 fp16 has steps of 2^-24 whatever the value: rounding is off by up to 2^-25 (3% of
+        # the mean output for values of 1e-6, so close()'s mean of relative errors does not apply).
+        # The other terms are close()'s.
+        want, spread, size, top = ref
+        tol = spread * (2 * 136 * 2.0 ** -24 * size + 1432 * 2.0 ** -24 + 4 * 2.0 ** -11 * size + 3 * 2.0 ** -11)
+        tol = tol + 700 * 2.0 ** -31 * top
+        tol = tol + 1.001 * 2.0 ** -11 * (want.abs() + tol) + 1.001 * 2.0 ** -25
+        assert ((got.double() - want).abs() <= tol).all()
+    else:
+        close(got, *ref, 128, 700, dtype)
+    assert torch.isfinite(out[3].float()).all()
+
+
+def test_garbage_behind_the_last_row():
+    s = Setup([(200, 300), (200, 264), (150, 249)] * 3, 16, 2, 128, 64, BF16, seed=2, width=8)
+    want = s.cache.attention(s.batch, s.q).clone()
+    used = torch.zeros(s.pages.shape[0], s.page, dtype=torch.bool)
+    for b, (_, r) in enumerate(s.seqs):
+        for i, p in enumerate(s.ids[b]):
+            used[p, :max(0, min(s.page, r - i * s.page))] = True
+    k, v = s.k.clone(), s.v.clone()
+    k[~used.cuda()], v[~used.cuda()] = float("nan"), float("nan")
+    s.pages.copy_(R.Cache(1, s.nkv, s.hd, s.page).pages(k, v))
+    for b in range(len(s.seqs)):
+        s.batch.page_table[b, len(s.ids[b]):] = torch.tensor([10 ** 9, -5, 77777, 2 ** 31 - 1])[:8 - len(s.ids[b])]
+    assert torch.equal(s.cache.attention(s.batch, s.q), want)
+    s.batch.check()
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_nan_rows_reach_the_rows_that_see_them(which):
+    """A block held as NaN at row 250 of the second sequence: tokens in front of it and other
+    sequences are as without it, those that see it are NaN (its 32 dimensions, for V)."""
+    s = Setup([(200, 300), (200, 300), (100, 600)] * 3, 16, 2, 128, 64, BF16, seed=5)
+    ref = s.expect()
+    x = (s.k if which == "k" else s.v).clone()
+    x[s.ids[1][250 // 64], 250 % 64, 1, 70] = float("nan")
+    s.pages.copy_(R.Cache(1, 2, 128, 64).pages(*((x, s.v) if which == "k" else (s.k, x))))
+    out = s.cache.attention(s.batch, s.q)
+    first = s.start[1] + 150   # the token of row 250
+    hit = torch.zeros(s.T, 16, 128, dtype=torch.bool, device="cuda")
+    hit[first:s.start[2], 8:] = True
+    if which == "v":
+        hit[..., :64], hit[..., 96:] = False, False
+    assert torch.isnan(out[hit]).all() and torch.isfinite(out[~hit].float()).all()
+    rest = [t for t in range(s.T) if not first <= t < s.start[2]]
+    close(out[rest], *[y[rest] for y in ref], 128, 600, BF16)
+    s.batch.check()
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 4, 64), (12, 4, 128)])
+def test_padding_strides_and_in_place(nh, nkv, hd):
+    s = Setup([(300, 390), (129, 130)] * 4, nh, nkv, hd, 32, BF16, seed=4, pad=70)
+    w, n = nh * hd, s.start[-1]
+    want = s.cache.attention(s.batch, s.q)
+    wide = torch.full((s.T, w + 260), 5.0, dtype=BF16, device="cuda")
+    wide[:, 132:132 + w] = s.q.flatten(1)
+    dst = torch.full((s.T, 3, w), 7.0, dtype=BF16, device="cuda")
+    s.cache.attention(s.batch, wide[:, 132:132 + w], out=dst[:, 1])
+    assert torch.equal(dst[:n, 1], want[:n].flatten(1))
+    assert (dst[n:] == 7).all() and (dst[:, 0] == 7).all() and (dst[:, 2] == 7).all()
+    s.cache.attention(s.batch, s.q, out=s.q)
+    assert torch.equal(s.q[:n], want[:n])
+
+
+def test_the_last_rows_of_the_last_page_of_memory():
+    """q and out that end with their allocation's last row, at every number of rows of an item's
+    second tile: what lies behind is neither read into results nor written."""
+    for n in (129, 135, 255):
+        s = Setup([(n, n)] * 16, 4, 4, 64, 16, BF16, seed=n)
+        guard = torch.full((s.T + 300, 256), float("nan"), dtype=BF16, device="cuda")
+        guard[:s.T] = s.q.flatten(1)
+        out = torch.full((s.T + 300, 256), 9.0, dtype=BF16, device="cuda")
+        s.cache.attention(s.batch, guard[:s.T], out=out[:s.T])
+        close(out[:s.T].view(s.T, 4, 64), *s.expect(), 64, n, BF16)
+        assert (out[s.T:] == 9).all()
+
+
+def test_faults_are_reported():
+    s = Setup([(150, 300), (150, 300), (130, 164)] * 3, 16, 2, 64, 16, BF16, seed=6)
+    table = s.batch.page_table.clone()
+    ref = s.expect()
+    s.batch.page_table[0, 2] = 12345            # rows 32 .. 47 of sequence 0 are left out
+    out = s.cache.attention(s.batch, s.q)
+    keep = [r for r in range(300) if not 32 <= r < 48]
+    one = R.attention(s.q[:150].double(), s.rows(0, s.hk)[keep], s.rows(0, s.hv)[keep], 0.125)
+    close(out[:150], *one, 64, 300, BF16)
+    close(out[150:], *[x[150:] for x in ref], 64, 300, BF16)
+    with pytest.raises(RuntimeError, match="page id"):
+        s.batch.check()
+    s.batch.page_table.copy_(table)
+    s.batch.kv_lens[1] = table.shape[1] * 16 + 50
+    s.cache.attention(s.batch, s.q)
+    with pytest.raises(RuntimeError, match="length"):
+        s.batch.check()
+    s.batch.kv_lens[1] = 300
+    from tinygiant_b200.paged import PagedBatch
+    few = PagedBatch(s.batch.q_start, s.batch.kv_lens, s.batch.page_table, 140)
+    dst = torch.full_like(s.q, 3.0)
+    s.cache.attention(few, s.q, out=dst)
+    with pytest.raises(RuntimeError, match="max_new"):
+        few.check()
+    for b, (n, _) in enumerate(s.seqs):
+        part = dst[s.start[b]:s.start[b + 1]]
+        assert (part[140:] == 3).all() and (part[:140] != 3).any(-1).all()
+
+
+def test_nonsense_starts_do_no_harm():
+    s = Setup([(140, 150), (140, 160), (140, 170)] * 2, 32, 4, 64, 16, BF16, seed=8)
+    for start in ([5, 0, 2 ** 31 - 1, 12, 700, 3, 800], [-2 ** 31, 2 ** 31 - 1, -1, 3, 0, 840, 0], [9] * 7,
+                  [0, 840, 0, 840, 0, 840, 0], [840, 700, 500, 300, 200, 100, 0]):
+        s.batch.q_start.copy_(torch.tensor(start, dtype=torch.int32))
+        for lens in ([150, 160, 170] * 2, [-2 ** 31, 2 ** 31 - 1, -1] * 2, [0, 1, 16] * 2):
+            s.batch.kv_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+            s.cache.attention(s.batch, s.q)
+    torch.cuda.synchronize()
+
+
+def test_equal_results_every_time():
+    s = Setup(MANY, 32, 4, 128, 64, F16, seed=11)
+    want = s.cache.attention(s.batch, s.q).clone()
+    for _ in range(200):
+        assert torch.equal(s.cache.attention(s.batch, s.q), want)
+
+
+def test_streams_and_two_graphs():
+    """Captured twice and replayed with other lengths, starts and queries; a third graph of few
+    tokens, on the same cache, in between."""
+    s = Setup([(200, 700), (200, 290), (200, 1000)], 32, 4, 128, 64, BF16, seed=17)
+    want = s.cache.attention(s.batch, s.q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = s.cache.attention(s.batch, s.q, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    outs, graphs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(s.cache.attention(s.batch, s.q))
+        graphs.append(g)
+    q2 = torch.randn_like(s.q)
+    for lens, start in (([200, 290, 264], [0, 200, 400, 600]), ([700, 264, 999], [0, 100, 101, 301]),
+                        ([0, 233, 500], [0, 0, 200, 400]), ([700, 290, 1000], [600, 600, 600, 600])):
+        s.batch.kv_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        s.batch.q_start.copy_(torch.tensor(start, dtype=torch.int32))
+        s.q.copy_(q2)
+        for g, o in zip(graphs, outs):
+            o.fill_(1)
+            g.replay()
+        ref = s.cache.attention(s.batch, s.q, out=torch.ones_like(s.q))
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], ref) and torch.equal(outs[1], ref)
+    s.batch.check()
