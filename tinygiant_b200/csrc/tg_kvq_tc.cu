@@ -38,7 +38,7 @@ namespace {
 constexpr int QT = 128;          // query rows of a tile
 constexpr int TK = 64;           // tokens of a tile: K or V of a granule per conversion warp
 constexpr int SLOTS = 6;
-constexpr int SW = 8, DW = 8;    // softmax and conversion warps; one more for the MMAs
+constexpr int SW = 8, DW = 8;    // softmax and conversion warps; four more, two of them for the MMAs
 constexpr int THREADS = 32 * (SW + DW + 4);
 constexpr float P_EXP = 6.0f, SLACK = 8.0f;   // p is held times 2^6, and up to 2^14: fp16 reaches 2^16
 
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
         mbar_init(&s_bars[0], 32 * SW);
         for (int i = 1; i < 7; i++) mbar_init(&s_bars[i], 1);
         for (int i = 7; i < 11; i++) mbar_init(&s_bars[i], QT);
-        for (int i = 0; i < SLOTS; i++) mbar_init(&s_bars[11 + i], 16 * DW), mbar_init(&s_bars[11 + SLOTS + i], 1);
+        for (int i = 0; i < SLOTS; i++) mbar_init(&s_bars[11 + i], 16 * DW), mbar_init(&s_bars[11 + SLOTS + i], 2);
         s_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;");
     }
@@ -495,14 +495,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == SW + DW && tiles) {
-            // ================================ the MMAs
+        if (warp < SW + DW + 2 && tiles) {
+            // ================================ the MMAs, a warp per query tile
+            const int q = __shfl_sync(0xffffffffu, warp, 0) - SW - DW;
             constexpr uint32_t IDESC_S = (1u << 4) | ((TK >> 3) << 17) | ((QT >> 4) << 24);
             constexpr uint32_t IDESC_O = (1u << 4) | ((HD >> 3) << 17) | ((QT >> 4) << 24);
             const uint64_t dq = sw128_desc(saddr(s_q)), dr = sw128_desc(saddr(ring));
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             // the warp is in step throughout; one lane issues
-            auto scores = [&](int q, int i, int slot, bool last) {
+            auto scores = [&](int i, int slot) {
                 const uint32_t d = tm + q * 128 + (i & 1) * TK;
                 const uint64_t x = dq + (q * Q_BYTES >> 4), y = dr + (slot * SLOT >> 4);
                 if (elect_one()) {
@@ -510,18 +511,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
                     for (int s = 0; s < 2 * NB; s++)
                         mma_f16_ss(d, x + ((s / 4 * ATOM + s % 4 * 32) >> 4), y + ((s / 4 * K_ATOM + s % 4 * 32) >> 4), IDESC_S, s > 0);
                     commit(s_full(q, i));
-                    if (last) commit(empty(slot));
+                    commit(empty(slot));
                 }
                 __syncwarp();
             };
-            auto values = [&](int q, int i, int slot, bool last) {
+            auto values = [&](int i, int slot) {
                 const uint32_t d = tm + 256 + q * 128, x = tm + q * 128 + (i & 1) * TK;
                 const uint64_t y = dr + (slot * SLOT >> 4);
                 if (elect_one()) {
 #pragma unroll
                     for (int s = 0; s < TK / 16; s++) mma_f16_ts(d, x + 8 * s, y + (s * 32 >> 4), IDESC_O, i > 0 || s > 0);
                     commit(pv_done(q));
-                    if (last) commit(empty(slot));
+                    commit(empty(slot));
                 }
                 __syncwarp();
             };
@@ -536,23 +537,20 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             bool good = wait(q_full, 0) && wait(full(0), 0);
             if (good) {
                 fence();
-                scores(0, 0, 0, false);
-                scores(1, 0, 0, true);
+                scores(0, 0);
                 step(kslot, kphase);
             }
             for (int i = 0; i < tiles && good; i++) {
-                const bool more = i + 1 < tiles;
-                if (more) good = wait(full(kslot), kphase);
-                for (int q = 0; q < 2 && good; q++) {
-                    if (more) {   // the next scores go into the other half of S, which O's last sum has read
-                        fence();
-                        scores(q, i + 1, kslot, q == 1);
-                    }
-                    good = (q || wait(full(vslot), vphase)) && wait(p_ready(q, i), i >> 1 & 1);
+                if (i + 1 < tiles) {   // the next scores go into the other half of S, which O's last sum has read
+                    good = wait(full(kslot), kphase);
                     if (!good) break;
                     fence();
-                    values(q, i, vslot, q == 1);
+                    scores(i + 1, kslot);
                 }
+                good = wait(full(vslot), vphase) && wait(p_ready(q, i), i >> 1 & 1);
+                if (!good) break;
+                fence();
+                values(i, vslot);
                 step(kslot, kphase);
                 step(vslot, vphase);
             }
