@@ -14,12 +14,15 @@
 // dimension for V.  The scores of a tile are issued before the softmax of the one in front is
 // waited for, so the softmax warps go from tile to tile.
 //
-// Three prompts of up to 1500 tokens behind up to 2500 (32 heads over 4 kv heads of 128): 156 us,
-// 1.1 us a pair of tiles of 64 tokens.  There the issue of the MMAs takes 1700 of 2350 cycles (24
-// of them, 70 cycles each; at N = 64 the tensor cores' own time is 1024), the softmax 1300.
-// 254 us with tiles of 128 tokens and one S per query tile; 246 with four conversion warps,
-// query rows read and written a row a thread (34000 cycles before the first tile, 9000 now), and
-// the items of a sequence next to one another instead of in order of the rows they see.
+// Three prompts of up to 1500 tokens behind up to 2500 (32 heads over 4 kv heads of 128): 139 us,
+// 10 of them k_kvq_scan's and 8 the empty pass of the other kernel.  A pair of tiles takes 1950
+// cycles: its MMAs about 64 each whether N is 64 or 128 (1536 in all), its exponentials 1024.
+// Measured on the way: 254 us with tiles of 128 tokens and one S per query tile; 246 with four
+// conversion warps, query rows read and written a row a thread (34000 cycles before the first
+// tile, 7000 now) and a sequence's items next to one another instead of in order of the rows they
+// see; 156 with one warp that issues for both query tiles.  Tiles of 128 tokens, which halve the
+// score MMAs, measured 157 to 183 us again: without a second S a query tile's softmax and MMAs
+// take turns.
 //
 // m moves, and O in TMEM is rescaled, only when a row's scores leave 2^SLACK of it.  q rows, K
 // and V are held in fp16 times powers of two: q's largest in 2^13 .. 2^14, the largest scale of
@@ -105,6 +108,31 @@ __global__ void __launch_bounds__(1024) k_kvq_scan(AttnKvqArgs a, int* marks, in
     __shared__ unsigned s_top[2];
     const int j = blockIdx.x, b = blockIdx.y, hd = a.c.hd, lb = hd == 128 ? 2 : 1;   // 2^lb blocks a row
     const SeqInfo si = seq_info(a, b, 2 * QT);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (j == a.c.nkv) {   // the items of the sequence, a warp each
+        const int lane = threadIdx.x & 31, rt_step = blockDim.x / 32;
+        for (int rt = threadIdx.x / 32; rt < si.tiles || (b == 0 && rt == threadIdx.x / 32); rt += rt_step) {
+            const int mine = rt < si.tiles ? item_seen(a, si, rt) : 0;
+            int rank = 0, all = 0;
+            for (int x = lane; x < a.b.B; x += 32) {
+                const SeqInfo sx = seq_info(a, x, 2 * QT);
+                int lo = 0, hi = sx.tiles;   // the first that is in front of mine: they see more and more
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1, see = item_seen(a, sx, mid);
+                    const bool front = see > mine || (see == mine && (x < b || (x == b && mid > rt)));
+                    if (front)
+                        hi = mid;
+                    else
+                        lo = mid + 1;
+                }
+                rank += sx.tiles - lo, all += sx.tiles;
+            }
+            rank = __reduce_add_sync(0xffffffffu, rank), all = __reduce_add_sync(0xffffffffu, all);
+            if (lane == 0 && rt < si.tiles && rank < cap) order[rank] = make_int2(b, rt);
+            if (threadIdx.x == 0 && b == 0) *items = min(all, cap);   // more than cap: q_start goes back
+        }
+        return;
+    }
     if (threadIdx.x < 2) s_top[threadIdx.x] = 0;
     __syncthreads();
     const int parts = 2 * hd / 16, gpp = a.c.pt >> 4;   // 16-byte parts of a granule's scales: K's, then V's
@@ -156,29 +184,6 @@ __global__ void __launch_bounds__(1024) k_kvq_scan(AttnKvqArgs a, int* marks, in
         if ((threadIdx.x & 31) == 0) atomicMax(&s_top[i], top[i]);
     }
     __syncthreads();
-    if (j == 0) {   // a warp per item
-        const int lane = threadIdx.x & 31, rt_step = blockDim.x / 32;
-        for (int rt = threadIdx.x / 32; rt < si.tiles || (b == 0 && rt == threadIdx.x / 32); rt += rt_step) {
-            const int mine = rt < si.tiles ? item_seen(a, si, rt) : 0;
-            int rank = 0, all = 0;
-            for (int x = lane; x < a.b.B; x += 32) {
-                const SeqInfo sx = seq_info(a, x, 2 * QT);
-                int lo = 0, hi = sx.tiles;   // the first that is in front of mine: they see more and more
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1, see = item_seen(a, sx, mid);
-                    const bool front = see > mine || (see == mine && (x < b || (x == b && mid > rt)));
-                    if (front)
-                        hi = mid;
-                    else
-                        lo = mid + 1;
-                }
-                rank += sx.tiles - lo, all += sx.tiles;
-            }
-            rank = __reduce_add_sync(0xffffffffu, rank), all = __reduce_add_sync(0xffffffffu, all);
-            if (lane == 0 && rt < si.tiles && rank < cap) order[rank] = make_int2(b, rt);
-            if (threadIdx.x == 0 && b == 0) *items = min(all, cap);   // more than cap: q_start goes back
-        }
-    }
     if (threadIdx.x == 0) {
         int e[2];
 #pragma unroll
@@ -212,6 +217,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     auto empty = [&](int slot) { return bars + 88 + 8 * SLOTS + 8 * slot; };
 
     const int item = blockIdx.x / a.c.nkv, j = blockIdx.x % a.c.nkv;   // the longest first
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (item >= *t.items) return;
     const int b = t.order[item].x, rt = t.order[item].y;
     const SeqInfo si = seq_info(a, b, 2 * QT);
@@ -578,8 +584,17 @@ cudaError_t launch_tc(const TcArgs& t, cudaStream_t s) {
     constexpr int smem = 2 * (NB / 2) * QT * 128 + SLOTS * 4096 * NB + 1024;
     cudaError_t e = cudaFuncSetAttribute(k_kvq_tc<DT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    k_kvq_tc<DT, NB><<<(unsigned)(item_cap(t.a.b, t.a.T, t.a.R) * t.a.c.nkv), THREADS, smem, s>>>(t);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(item_cap(t.a.b, t.a.T, t.a.R) * t.a.c.nkv));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_kvq_tc<DT, NB>, t);
 }
 
 }  // namespace
@@ -608,7 +623,7 @@ cudaError_t launch_attn_tc(int dtype, const AttnKvqArgs& a, void* scratch, const
     int2* exps = (int2*)take((size_t)a.c.nkv * a.b.B * 8);
     int2* order = (int2*)take((size_t)cap * 8);
     int* items = (int*)take(4);
-    k_kvq_scan<<<dim3(a.c.nkv, a.b.B), 1024, 0, s>>>(a, marks, exps, order, items, cap);
+    k_kvq_scan<<<dim3(a.c.nkv + 1, a.b.B), 1024, 0, s>>>(a, marks, exps, order, items, cap);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const TcArgs t{a, marks, exps, order, items};
