@@ -233,7 +233,7 @@ def test_steps_with_experts_and_generation():
         assert toks == said[i], i
     assert len(list(eng.generate(prompts, 2, temperature=0.8, rng=np.random.RandomState(1)))) == 2
     for bad in (dict(prompts=[[1], []]), dict(prompts=[]), dict(n_tokens=0), dict(prompts=[[1] * 60], n_tokens=6),
-                dict(prompts=[[1] * 40] * 9, n_tokens=6)):
+                dict(prompts=[[1] * 40] * 9, n_tokens=6), dict(prompts=[[300]]), dict(prompts=[[-1]])):
         with pytest.raises(ValueError):
             next(eng.generate(**{**dict(prompts=prompts, n_tokens=4), **bad}))
     m.close()
@@ -275,3 +275,22 @@ def test_rows_that_are_not_finite_keep_to_themselves():
         keep = [i for i in range(9) if i != 4]
         assert torch.equal(X[keep], Y[keep]) and torch.isnan(Y[4]).any()
     m.close()
+
+
+def test_step_with_tokens_and_starts_that_do_not_fit():
+    """Ids outside the vocabulary and starts behind the last token reach no memory outside."""
+    from tinygiant_b200.serving import BatchedAttention, BatchedEngine
+    a = BatchedAttention(64, 2, 1, 64, 1, 8, 16, 64)
+    a.fill_synthetic(1)
+    eng = BatchedEngine.synthetic(None, a, 50, 2)
+    want = eng.step(batch_of([(2, 2), (1, 1)], width=4), torch.tensor([49, 0, 7], device="cuda"))
+    got = eng.step(batch_of([(2, 2), (1, 1)], width=4), torch.tensor([2 ** 40, -3, 7], device="cuda"))
+    assert torch.equal(got, want)
+    out = eng.step(batch_of([(2, 2), (9, 9)], width=4), torch.tensor([49, 0, 7], device="cuda"))
+    assert out.shape == (2, 50) and torch.equal(out[0], want[0])
+    for bad in (torch.zeros(0, dtype=torch.long, device="cuda"), torch.zeros(1, 1, dtype=torch.long, device="cuda"),
+                torch.zeros(2, dtype=torch.long)):
+        with pytest.raises(ValueError):
+            eng.step(batch_of([(1, 1)], width=4), bad)
+    with pytest.raises(ValueError):
+        BatchedEngine(None, a, torch.zeros(49, 64), torch.ones(64), torch.zeros(50, 64))

@@ -850,10 +850,13 @@ struct Shape {
     int wide;   // items for the wide join, 0 for the other
 };
 
+// Query rows per kv head that the launch is made for.  Behind the tiles of tg_kvq_tc.cu these are a
+// decode step's (sequences that it leaves for their scales may have more, and take longer).
+long long shape_rows(const KvqBatch& b, int R, bool left) { return left ? R : (long long)b.max_new * R; }
+
 // Workers and their row tiles for these bounds; at most `have` workers are resident.
-Shape shape_of(const KvqCache& c, const KvqBatch& b, int R, bool two, int have_one, int have_deep) {
+Shape shape_of(const KvqCache& c, const KvqBatch& b, long long rows, bool left, bool two, int have_one, int have_deep) {
     Shape sh;
-    const long long rows = (long long)b.max_new * R;
     sh.warps = rows <= DEEP_ROWS ? DEEP_WARPS : 1;
     sh.nt = rows > 8 && two ? 2 : 1;
     // no more workers than there can be granules for their warps
@@ -862,7 +865,7 @@ Shape shape_of(const KvqCache& c, const KvqBatch& b, int R, bool two, int have_o
     const long long have = sh.warps > 1 ? have_deep : have_one, want = (most + sh.warps - 1) / sh.warps;
     sh.workers = (int)(want < have ? want : have);
     // many parts per item: 14 us -> see k_kvq_join_wide
-    sh.wide = items * 16 < sh.workers ? (int)items : 0;
+    sh.wide = items * 16 < sh.workers && !left ? (int)items : 0;   // a bound on the items, so not for what is left
     return sh;
 }
 
@@ -913,11 +916,11 @@ cudaError_t launch_attn_t(AttnKvqArgs a, const Shape& sh, cudaStream_t s) {
 template <int DT, int NB>
 cudaError_t launch_attn_nb(AttnKvqArgs a, void* scratch, size_t scratch_bytes, cudaStream_t s) {
     constexpr int NT2 = two_tiles(DT, NB) ? 2 : 1;
-    const bool nt2 = NT2 == 2 && (long long)a.b.max_new * a.R > 8;
+    const bool left = a.only != nullptr, nt2 = NT2 == 2 && shape_rows(a.b, a.R, left) > 8;
     const int one = nt2 ? attn_workers<DT, NB, NT2>(1) : attn_workers<DT, NB, 1>(1);
     const int deep = nt2 ? attn_workers<DT, NB, NT2>(DEEP_WARPS) : attn_workers<DT, NB, 1>(DEEP_WARPS);
     if (!one || !deep) return cudaErrorUnknown;
-    const Shape sh = shape_of(a.c, a.b, a.R, NT2 == 2, one, deep);
+    const Shape sh = shape_of(a.c, a.b, shape_rows(a.b, a.R, left), left, NT2 == 2, one, deep);
     if (scratch_bytes < attn_scratch(sh, a.c.hd)) return cudaErrorInvalidValue;
     a.heads = reinterpret_cast<int*>(scratch);
     a.slots = reinterpret_cast<float*>((uint8_t*)scratch + head_bytes(sh.workers));
@@ -965,11 +968,14 @@ extern "C" size_t tgx_kvq_attention_scratch_bytes(const tgx_kvq_cache* cache, co
         return 0;
     const tg::KvqCache c = tg::kvq_cache(*cache);
     const tg::KvqBatch b = tg::kvq_batch(*batch);
+    const int R = n_heads / c.nkv;
     size_t most = 0;   // of any type, on any device
     for (int two = 0; two < 2; two++)
-        most = std::max(most, tg::attn_scratch(tg::shape_of(c, b, n_heads / c.nkv, two, tg::MAX_SMS * tg::workers_per_sm(1),
-                                                            tg::MAX_SMS * tg::workers_per_sm(tg::DEEP_WARPS)), c.hd));
-    return most + tg::attn_tc_scratch(c, b, n_tokens, n_heads / c.nkv);
+        for (int left = 0; left < 2; left++)
+            most = std::max(most, tg::attn_scratch(tg::shape_of(c, b, tg::shape_rows(b, R, left), left, two,
+                                                                tg::MAX_SMS * tg::workers_per_sm(1),
+                                                                tg::MAX_SMS * tg::workers_per_sm(tg::DEEP_WARPS)), c.hd));
+    return most + tg::attn_tc_scratch(c, b, n_tokens, R);
 }
 
 extern "C" int tgx_kvq_attention(const tgx_kvq_cache* cache, const tgx_kvq_batch* batch, int dtype, int n_tokens,

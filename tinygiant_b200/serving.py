@@ -117,6 +117,8 @@ class BatchedEngine:
         self.head = output_weight if isinstance(output_weight, Int8Linear) else \
             Int8Linear.quantize(output_weight.to(attn.device))
         self.vocab = self.head.out_features
+        if self.embd.shape[0] != self.vocab or self.head.in_features != attn.embed or self.norm.shape != (attn.embed,):
+            raise ValueError("embeddings, output norm and output weights differ in size")
 
     @classmethod
     def synthetic(cls, moe: MoEModel | None, attn: BatchedAttention, vocab: int, seed: int):
@@ -127,13 +129,15 @@ class BatchedEngine:
 
     def step(self, batch: PagedBatch, tokens, stream=None):
         """Logits float32 [B][vocab] behind each sequence's last new token; tokens: int [T] on the
-        device, the batch's new tokens in its rows' order.  The row of a sequence without new
-        tokens says nothing."""
+        device, the batch's new tokens in its rows' order (an id outside the vocabulary counts as
+        the nearest in it).  The row of a sequence without new tokens says nothing."""
         if stream is not None:
             with on_stream(stream, self.attn.device):
                 return self.step(batch, tokens)
-        X = self.attn.forward(batch, self.embd.index_select(0, tokens), self.moe)
-        last = (batch.q_start[1:] - 1).clamp(min=0)
+        if tokens.dim() != 1 or not tokens.numel() or tokens.device != self.attn.device:
+            raise ValueError(f"tokens: expected at least one, in a row on {self.attn.device}")
+        X = self.attn.forward(batch, self.embd.index_select(0, tokens.clamp(0, self.vocab - 1)), self.moe)
+        last = (batch.q_start[1:] - 1).clamp(0, X.shape[0] - 1)
         return self.head(X.index_select(0, last), norm=self.norm, eps=self.attn.eps)
 
     def generate(self, prompts, n_tokens: int = 128, temperature: float = 0.7, top_p: float = 0.9, rng=np.random):
@@ -144,6 +148,8 @@ class BatchedEngine:
         lens = [len(p) for p in prompts]
         if not lens or min(lens) < 1 or n_tokens < 1:
             raise ValueError("expected prompts of at least one token, and tokens to generate")
+        if any(not 0 <= t < self.vocab for p in prompts for t in p):
+            raise ValueError(f"a token outside the vocabulary of {self.vocab}")
         if max(lens) + n_tokens - 1 > self.attn.cos.shape[0]:
             raise ValueError(f"positions up to {max(lens) + n_tokens - 1}: the rope tables end at {self.attn.cos.shape[0]}")
         need = [-(-(n + n_tokens - 1) // pt) for n in lens]
