@@ -94,10 +94,10 @@ __device__ __forceinline__ void i8_codes(uint32_t (&c)[V / 4], const float (&x)[
 // over it beat rows held in registers, whose unrolled code did not fit the instruction cache
 // (8100 x 2048 bf16 behind a norm: 41 to 56 us).
 //
-// Bound by the instructions, about 15 an element, for many rows: a warp each and no barrier
+// Bound by the instructions, about 20 an element, for many rows (8100 x 2048: 23 us): a warp each and no barrier
 // (G = 1).  For few rows, by latency: a CTA each (G = 8).
 template <int DT, bool NORM, bool VEC, int G>
-__global__ void __launch_bounds__(256) k_i8_rows(QuantArgs a) {
+__global__ void __launch_bounds__(256, 4) k_i8_rows(QuantArgs a) {
     using T = typename Elem<DT>::T;
     constexpr int V = 16 / sizeof(T), NT = 32 * G;
     static_assert(G == 1 || G == 8, "a warp or a CTA of 256 threads per row");
@@ -161,13 +161,23 @@ __global__ void __launch_bounds__(256) k_i8_rows(QuantArgs a) {
     if (NORM && hi > 0.0f && !poor) {
         double y = 0.0;   // the largest in 64 bits, where it may be
         exact = hi < 1e-30f;   // what such products lose is beyond fp32, too
-        if (own == hi || exact)
-            each([&](const float (&v)[V], const float (&w)[V], int, int at) {
-                if ((where >> at & 1) || exact)
+        auto largest = [&](const float (&v)[V], const float (&w)[V]) {
 #pragma unroll
-                    for (int i = 0; i < V; i++)
-                        if (exact || fabsf(__fmul_rn(v[i], w[i])) == hi) y = fmax(y, fabs((double)v[i] * w[i]));
-            });
+            for (int i = 0; i < V; i++)
+                if (exact || fabsf(__fmul_rn(v[i], w[i])) == hi) y = fmax(y, fabs((double)v[i] * w[i]));
+        };
+        if (exact || (own == hi && where >> 31)) {
+            each([&](const float (&v)[V], const float (&w)[V], int, int) { largest(v, w); });
+        } else if (own == hi) {   // few pieces, mostly one
+#pragma unroll 1
+            for (uint32_t left = where; left; left &= left - 1) {
+                const int c = (tid + (__ffs(left) - 1) * NT) * V;
+                float v[V], w[V];
+                load_piece<false>(v, x, c, a.cols);
+                load_norm<NORM, false>(w, a.norm, c, a.cols);
+                largest(v, w);
+            }
+        }
         __syncwarp();
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) y = fmax(y, __shfl_xor_sync(0xffffffffu, y, o));
