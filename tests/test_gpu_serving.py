@@ -294,3 +294,24 @@ def test_step_with_tokens_and_starts_that_do_not_fit():
             eng.step(batch_of([(1, 1)], width=4), bad)
     with pytest.raises(ValueError):
         BatchedEngine(None, a, torch.zeros(49, 64), torch.ones(64), torch.zeros(50, 64))
+
+
+def test_two_streams_at_once():
+    """Prompts on one stream and single tokens on another, each on its own cache, over and over: the
+    same bits as one after the other."""
+    from tests.test_gpu_kvq import Setup
+    from tinygiant_b200.int8 import Int8Linear
+    p = Setup([(300, 900), (257, 257), (90, 1200)], 32, 4, 128, 64, BF16, seed=1)
+    d = Setup([(1, 700 + 13 * i) for i in range(24)], 32, 4, 128, 64, BF16, seed=2)
+    lin = Int8Linear.quantize(torch.randn(1000, 640, generator=gen(3), device="cuda"))
+    x = torch.randn(700, 640, generator=gen(4), device="cuda")
+    want = [p.cache.attention(p.batch, p.q), lin(x), d.cache.attention(d.batch, d.q), lin(x[:5])]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        got.append((p.cache.attention(p.batch, p.q, stream=streams[0]), lin(x, stream=streams[0]),
+                    d.cache.attention(d.batch, d.q, stream=streams[1]), lin(x[:5], stream=streams[1])))
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
