@@ -162,3 +162,27 @@ def test_streams_and_graphs(m):
         g.replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], ref) and torch.equal(outs[1], ref)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m,n,k", [(2100, 8449, 2048), (2177, 8500, 100), (4097, 4700, 31), (2305, 8193, 16), (76000, 100, 130),
+                                   (300, 38000, 500)])
+def test_product_of_many_tiles(m, n, k, dtype):
+    """Tokens and channels for several rounds of the largest tiles, whose last ones are nearly empty."""
+    from tinygiant_b200.int8 import Int8Linear
+    lin = Int8Linear.quantize(randn(1, n, k) * 0.05)
+    x = (randn(2, m, k) * 2).to(dtype)
+    got = check(x, lin)
+    if dtype == BF16:
+        check(x, lin, norm=1 + 0.2 * randn(3, k), residual=randn(4, m, n).to(dtype))
+        wide = torch.full((m, n + 3), 7.0, dtype=dtype, device="cuda")   # rows on no vector boundary
+        lin(x, out=wide[:, 1:n + 1])
+        assert torch.equal(wide[:, 1:n + 1], got) and (wide[:, 0] == 7).all() and (wide[:, n + 1:] == 7).all()
+        graph, y = torch.cuda.CUDAGraph(), torch.empty_like(got)
+        with torch.cuda.graph(graph):
+            lin(x, out=y)
+        x.mul_(0.5)   # the codes stay, the scales halve
+        for _ in range(3):
+            y.fill_(1)
+            graph.replay()
+            assert torch.equal(y, lin(x))

@@ -228,7 +228,9 @@ __global__ void __launch_bounds__(256, 4) k_i8_rows(QuantArgs a) {
 // finishes every splits-th column, exactly, whatever the split.
 //
 // Many tokens (8100 x 5120 x 2048: 64 us, 2.6 Pop/s) are bound by the operands' way from L2: a
-// stage is 48 KB for 512 cycles of MMAs, 15.6 TB/s over all SMs, 62 bytes a cycle and SM.
+// stage is 48 KB for 512 cycles of MMAs, 15.6 TB/s over all SMs, 62 bytes a cycle and SM.  Pairs
+// of CTAs on tiles of 256 x 256 (cta_group::2, 32 KB a stage, the second CTA passing on its full
+// barriers by remote arrivals) were right but took 136 us.
 //
 // The first copies of weights are issued before the quantiser in front has finished.
 // Every wait is bounded; where one expires the tile's outputs become NaN, copies and MMAs in
@@ -387,7 +389,7 @@ __global__ void __launch_bounds__(GT, 1)
             float* sa = s_sa[i & 1];   // the other one may still be read
             if (tid < g.tn) sa[tid] = m0 + tid < g.M ? g.sa[m0 + tid] : 0.0f;
             asm volatile("bar.sync 1, %0;" ::"n"(32 * EW) : "memory");
-            const bool ok = mbar_wait(&acc_full[i & 1], (i >> 1) & 1, failed);
+            const bool ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[i & 1], (i >> 1) & 1, failed));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t d = tmem + (i & 1) * (cols / 2) + ((uint32_t)(32 * quad) << 16);
             if (g.splits > 1) {
