@@ -206,3 +206,14 @@ def test_streams_and_two_graphs():
         torch.cuda.synchronize()
         assert torch.equal(outs[0], ref) and torch.equal(outs[1], ref)
     s.batch.check()
+
+
+@pytest.mark.parametrize("seqs", [[(32, 3000)] * 40 + [(1000, 1000)], [(256, 256)] * 40, [(40, 64)] * 100])
+def test_waits_end_whatever_the_warps_pace(seqs):
+    """Thousands of items: a wait that misses its phase ends after a second with NaN."""
+    s = Setup(seqs, 32, 4, 128, 64, BF16, seed=13)
+    want = s.cache.attention(s.batch, s.q).clone()
+    bad = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(1500):
+        bad += (s.cache.attention(s.batch, s.q) != want).sum()
+    assert torch.isfinite(want.float()).all() and int(bad) == 0

@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     constexpr int HD = 32 * NB, ATOM = QT * 128;               // bytes of 64 dimensions of 128 rows
     constexpr int Q_BYTES = NB / 2 * ATOM, SLOT = 4096 * NB, K_ATOM = TK * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t s_bars[11 + 2 * SLOTS];
+    __shared__ __align__(8) uint64_t s_bars[13 + 2 * SLOTS];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
     __shared__ __align__(4) uint8_t s_valid[8][TK / 16];   // [tile % 8]: whether its granules exist
@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     auto p_ready = [&](int q, int i) { return bars + 56 + 16 * q + 8 * (i & 1); };
     auto full = [&](int slot) { return bars + 88 + 8 * slot; };
     auto empty = [&](int slot) { return bars + 88 + 8 * SLOTS + 8 * slot; };
+    auto o_done = [&](int q) { return bars + 88 + 16 * SLOTS + 8 * q; };   // O's last sum
 
     const int item = blockIdx.x / a.c.nkv, j = blockIdx.x % a.c.nkv;   // the longest first
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
         for (int i = 1; i < 7; i++) mbar_init(&s_bars[i], 1);
         for (int i = 7; i < 11; i++) mbar_init(&s_bars[i], QT);
         for (int i = 0; i < SLOTS; i++) mbar_init(&s_bars[11 + i], 16 * DW), mbar_init(&s_bars[11 + SLOTS + i], 2);
+        for (int i = 0; i < 2; i++) mbar_init(&s_bars[11 + 2 * SLOTS + i], 1);
         s_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;");
     }
@@ -371,10 +373,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             mbar_arrive(p_ready(q, i));
         }
-        // The sums of the last two tiles, one by one: this warp's scores may have come before another
-        // warp's p of the tile in front, and a parity tells neighbouring phases apart, no more.
-        for (int i = max(0, tiles - 2); i < tiles && good; i++)
-            good = __all_sync(0xffffffffu, mbar_wait(pv_done(q), i & 1, failed));
+        // a barrier of its own: a parity of pv_done's tells neighbouring phases apart, and this warp may be
+        // two ahead of it (another's p of the tile in front is missing) or two behind
+        if (good && tiles) good = __all_sync(0xffffffffu, mbar_wait(o_done(q), 0, failed));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inv = !good ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
         const float v2 = pow2(ex.y);
@@ -533,6 +534,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
 #pragma unroll
                     for (int s = 0; s < TK / 16; s++) mma_f16_ts(d, x + 8 * s, y + (s * 32 >> 4), IDESC_O, i > 0 || s > 0);
                     commit(pv_done(q));
+                    if (i + 1 == tiles) commit(o_done(q));
                     commit(empty(slot));
                 }
                 __syncwarp();
