@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
 #pragma unroll
             for (int i = 0; i < (U * C + 31) / 32; i++) {
                 const int o = 32 * i + lane;
-                const int first = 32 * i / C, last = min(U * C - 1, 32 * i + 31) / C;   // granules of this round
+                const int first = 32 * i / C, last = min(U * C - 1, 32 * i + 31) / C;   // granules of the lanes
                 const int u = first == last ? first : o >= last * C ? last : first;
                 const uint8_t* from = (first == last ? src[first] : o >= last * C ? src[last] : src[first]) + 16 * (o - u * C);
                 const uint32_t n = first == last ? size[first] : o >= last * C ? size[last] : size[first];
