@@ -408,7 +408,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
         }
     } else if (warp < SW + DW) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         // ================================ codes into operands: K's or V's of a granule per warp and tile
         const int dw = warp - SW, gt = dw & 3, g = lane >> 2, c = lane & 3, gpp = a.c.pt >> 4;
         const bool is_v = dw >= DW / 2;
