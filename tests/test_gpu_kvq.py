@@ -171,6 +171,41 @@ def test_garbage_behind_the_last_row(new):
     s.batch.check()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("nh,nkv,hd,page", [(8, 2, 128, 64), (6, 2, 96, 32), (32, 1, 64, 16)])
+def test_large_values_behind_the_last_row(nh, nkv, hd, page, new, dtype):
+    """What a page held before: finite values with the largest scales, behind a sequence's last row
+    and in rows that it does not hold, change no bit of the outputs."""
+    s = Setup([(new, 100), (new, 64), (new, 49), (new, 333)], nh, nkv, hd, page, dtype, seed=2, values=0.05)
+    want = s.cache.attention(s.batch, s.q)
+    used = torch.zeros(s.pages.shape[0], s.page, dtype=torch.bool)
+    for b, (_, r) in enumerate(s.seqs):
+        for i, p in enumerate(s.ids[b]):
+            used[p, :max(0, min(s.page, r - i * s.page))] = True
+    k, v = s.k.clone(), s.v.clone()
+    k[~used.cuda()], v[~used.cuda()] = 5e5, -5e5   # scales of 62500
+    s.pages.copy_(R.Cache(1, s.nkv, s.hd, s.page).pages(k, v))
+    assert torch.equal(s.cache.attention(s.batch, s.q), want)
+    close(want, *s.expect(), hd, 333, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_large_values_that_no_query_of_a_tile_sees(dtype):
+    """Rows of a sequence behind all the queries of a tile are nothing to it, however large."""
+    s = Setup([(64, 64), (64, 90)], 8, 2, 128, 64, dtype, seed=3, values=0.05)
+    want = s.cache.attention(s.batch, s.q)
+    v = s.v.clone()
+    for b, (n, r) in enumerate(s.seqs):
+        for row in range(r - 32, r):   # the second half of the new tokens
+            v[s.ids[b][row // s.page], row % s.page] = -5e5
+    s.pages.copy_(R.Cache(1, s.nkv, s.hd, s.page).pages(s.k, v))
+    got = s.cache.attention(s.batch, s.q)
+    for b in range(2):
+        first = s.start[b]
+        assert torch.equal(got[first:first + 32], want[first:first + 32])
+
+
 def test_nan_rows_attended_give_nan():
     s = Setup([(1, 40)], 2, 1, 64, 16, F32)
     v = s.v.clone()

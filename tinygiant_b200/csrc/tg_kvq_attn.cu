@@ -13,8 +13,8 @@
 // fp32 inputs keep 22 bits of q and of p * d as two fp16 pieces, each an mma of its own; for
 // 16-bit types one piece (11 bits) is as fine as the output.  The pieces stay in fp16's range
 // by powers of two: q's rows are scaled to 2^13 .. 2^14, p to 2^6 at its maximum, V scales to
-// 2^2 .. 2^5 at the largest met so far (vexp; O is rescaled when a larger one comes).  So a
-// probability below 2^-31 of its row's largest counts as 0.
+// 2^2 .. 2^5 at the largest met so far among the rows that the item sees (vexp; O is rescaled when
+// a larger one comes).  So a probability below 2^-31 of its row's largest counts as 0.
 //
 // Codes become fp16 by masks: a nibble in the low bits of 1024, and one half-precision
 // operation makes it code - 8.  K's codes with 16-bit types go without the second: a nibble
@@ -444,6 +444,18 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
             float t[U][NT][4];
             constexpr uint32_t ALL = (1u << U) - 1;
             const bool edge = t0 + 16 * U > lim_min || (have & ALL) != ALL;
+            if (edge) {
+                // V scales that no row of the item sees (an earlier use of the page may have left them) become
+                // 0: they must neither choose vexp nor, beyond fp16 in its units, meet a probability of 0
+                const int left = s_lim[nrows - 1] - t0;
+#pragma unroll 1
+                for (int x = lane; x < U * 8 * NB; x += 32) {   // a word holds two tokens'
+                    const int u = x / (8 * NB), at = x - u * 8 * NB, seen = left - (16 * u + at / NB * 2);
+                    uint32_t* v = reinterpret_cast<uint32_t*>(ring + (k % ST) * (U * GB) + u * GB + 17 * HD) + at;
+                    if (seen < 2) *v = seen == 1 ? *v & 0xffffu : 0u;
+                }
+                __syncwarp();
+            }
             auto sees = [&](int u, int n, int x) {   // whether the column's row attends to the lane's token
                 return t0 + 16 * u + g + 8 * (x >> 1) < lim[n][x & 1] && (have >> (U - 1 - u) & 1);
             };
