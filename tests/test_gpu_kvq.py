@@ -401,6 +401,52 @@ def test_append_ties_zeros_and_values_out_of_range():
     assert torch.equal(s.pages, pages)
 
 
+@pytest.mark.parametrize("hd,gap", [(64, 4), (128, 8), (256, 16), (32, 2), (96, 6)])
+def test_append_keys_that_are_equal_in_32_bits_only(hd, gap):
+    """Two rotated keys of one block that 32 bits round to the same magnitude: the larger of the
+    exact ones gives the block its scale, whichever comes first."""
+    s = Setup([(8, 8)], 1, 1, hd, 16, F32, seed=1)
+    g, h = s.g, hd // 2
+    cos, sin = torch.full((8, h), 0.50000006, device="cuda"), torch.zeros(8, h, device="cuda")
+    lo, hi = 2 - 2.0 ** -22, 2 - 2.0 ** -23      # their products with the cosine: below and above 1
+    k, v = torch.zeros(8, hd, device="cuda"), torch.randn(8, hd, generator=g, device="cuda")
+    k[:, 32::32] = 2.0                           # blocks without a doubt
+    for t, (a, b, at) in enumerate([(lo, -hi, 0), (hi, -lo, 0), (-lo, hi, 0), (lo, hi, 0), (-hi, lo, 0), (lo, -hi, 1),
+                                    (-lo, hi, h % 32), (hi, -hi, 1)]):
+        k[t, at], k[t, at + gap] = a, b
+    pages = append_expect(s, v, k, v, cos, sin, None, None, 0.0, s.pages)[1]
+    s.cache.append(s.batch, None, k, v, cos, sin)
+    assert torch.equal(s.pages, pages)
+
+
+@pytest.mark.parametrize("size", [1.0, 1.37, 40.0, 1000.0])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_append_keys_that_the_rotation_cancels(hd, size):
+    """Blocks that come out of the rotation far smaller than they went in, whose roundings are those
+    of the large products; tables with an attention factor folded in."""
+    n, h = 512, hd // 2
+    s = Setup([(n, n)], 1, 1, hd, 64, F32, seed=hd)
+    turn = torch.rand(n, h, generator=s.g, device="cuda", dtype=torch.float64) * 1.2 + 0.2
+    cos, sin = (size * turn.cos()).float(), (size * turn.sin()).float()
+    depth = 10.0 ** (-6 * torch.rand(n, 1, generator=s.g, device="cuda", dtype=torch.float64) - 0.5)
+    k = torch.cat((turn.sin() + depth * torch.randn(n, h, generator=s.g, device="cuda", dtype=torch.float64), turn.cos()),
+                  1).float()
+    v = torch.randn(n, hd, generator=s.g, device="cuda")
+    pages = append_expect(s, v, k, v, cos, sin, None, None, 0.0, s.pages)[1]
+    s.cache.append(s.batch, None, k, v, cos, sin)
+    assert torch.equal(s.pages, pages)
+
+
+def test_append_keys_whose_squares_vanish():
+    """eps 0 and keys so small that fp32 squares are subnormal or 0: the norm is still the exact one's."""
+    s = Setup([(96, 96)], 2, 2, 128, 64, F32, seed=5)
+    q, k, v, cos, sin, qn, kn = append_case(s)
+    k = k * 10.0 ** torch.linspace(-17, -37, 96, device="cuda")[:, None]
+    pages = append_expect(s, q, k, v, cos, sin, qn, kn, 0.0, s.pages)[1]
+    s.cache.append(s.batch, None, k, v, cos, sin, qn, kn, eps=0.0)
+    assert torch.equal(s.pages, pages)
+
+
 def test_offsets_beyond_32_bits():
     """Pages whose bytes lie behind the first 4 GB of the cache."""
     from tinygiant_b200.paged import PagedBatch, PagedKV4

@@ -74,34 +74,39 @@ __device__ __forceinline__ float max_nan(float x, float y) {   // NaN if either 
     return z;
 }
 
-// x: the lane's N dimensions of a head of 16 lanes; w: their norm weights, or null.
+// x: the lane's N dimensions of a head of 16 lanes; w: their norm weights, or null.  Returns the
+// mean square plus eps (1 without a norm).
 template <int N, typename T>
-__device__ __forceinline__ void norm_head(T (&x)[N], const float* w, float eps) {
-    if (!w) return;
+__device__ __forceinline__ T norm_head(T (&x)[N], const float* w, float eps) {
+    if (!w) return 1;
     T ss = 0;
 #pragma unroll
     for (int i = 0; i < N; i++) ss += x[i] * x[i];
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const T r = inv_sqrt(ss / (16 * N) + (T)eps);
+    const T mean = ss / (16 * N) + (T)eps, r = inv_sqrt(mean);
     float wn[N];
     load_row(wn, w);
 #pragma unroll
     for (int i = 0; i < N; i++) x[i] = x[i] * r * (T)wn[i];
+    return mean;
 }
-// cs / sn: the lane's angles.
+// cs / sn: the lane's angles.  Returns the largest magnitude of the lane's cosines and sines, 1 at least.
 template <int N, typename T>
-__device__ __forceinline__ void rotate_head(T (&x)[N], const float* cs, const float* sn, int lane) {
-    if (!cs) return;
-    float c[N], s[N];
+__device__ __forceinline__ float rotate_head(T (&x)[N], const float* cs, const float* sn, int lane) {
+    if (!cs) return 1.0f;
+    float c[N], s[N], most = 1.0f;
     load_row(c, cs);
     load_row(s, sn);
+#pragma unroll
+    for (int i = 0; i < N; i++) most = fmaxf(most, fmaxf(fabsf(c[i]), fabsf(s[i])));
 #pragma unroll
     for (int i = 0; i < N; i++) {
         const T y = __shfl_xor_sync(0xffffffffu, x[i], 8);
         const T a = x[i] * (T)c[i], b = y * (T)s[i];
         x[i] = lane & 8 ? a + b : a - b;
     }
+    return most;
 }
 
 // A code is left in the low bits of 1.5 * 2^23 + code.  Packs a lane's N of them, elements N q and
@@ -170,14 +175,14 @@ __device__ __forceinline__ uint16_t quant_block(const T (&x)[N], int lane, uint3
     const bool bad = !(top <= 3.4028235e38f) || __hisinf(d), plain = !bad && top > 0.0f;
     float wide = 0.0f;   // how far a quotient may be off, beside its own roundings
     if constexpr (FUZZY) {
-        // off bounds the roundings of each value; their common factor, 1e-6
-        wide = off * __fdiv_rn(8.0f, top);
+        // off bounds the roundings of each value, x's and m's; their common factor, 1e-6
+        wide = off * __fdiv_rn(16.0f, top);
         const float lo = top * (1.0f - 1e-6f) - off, hi = top * (1.0f + 1e-6f) + off;
         int count = 0;
 #pragma unroll
         for (int i = 0; i < N; i++) count += fabsf(f[i]) >= top - 2.0f * off;
-        // of its rivals one in another lane shows there
-        again = count > 1 || (count == 1 && !has) || !plain || !(top > 1e-20f) ||
+        // rivals of the largest in other lanes: smaller ones show there, equal ones here
+        again = count > 1 || (count == 1 && !has) || __popc(who) > 1 || !plain || !(top > 1e-20f) ||
                 __half_as_ushort(__float2half_rn(lo * 0.125f)) != __half_as_ushort(__float2half_rn(hi * 0.125f));
     }
     constexpr float MAGIC = 12582912.0f;
@@ -281,17 +286,19 @@ __device__ __forceinline__ void key_head(const float (&x)[2 * NB], const float* 
         float y[N], top = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; i++) y[i] = x[i];
-        norm_head(y, w, eps);
+        const float mean = norm_head(y, w, eps);
 #pragma unroll
         for (int i = 0; i < N; i++) top = fmaxf(top, fabsf(y[i]));
+        top *= rotate_head(y, cs, sn, lane);
 #pragma unroll
         for (int o = 8; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        rotate_head(y, cs, sn, lane);
         // a value's roundings, each 2^-24: two of the norm on both of the pair (at most top each),
-        // two products, a sum of up to 1.5 top: 2 * 3 + 1.5 of them, less than 5e-7 top
+        // two products, a sum of up to 1.5 top: 2 * 3 + 1.5 of them, less than 5e-7 top, where top
+        // has the largest cosine or sine as a factor if that is above 1
         uint32_t word[4];
         const uint16_t d = quant_block<N, L, true>(y, lane, word, 5e-7f * top, again);
-        again = __any_sync(0xffffffffu, again);
+        // squares next to the smallest numbers have roundings beyond the common factor's 1e-6
+        again = __any_sync(0xffffffffu, again || !(mean > 1e-30f));
         if (!again && put) put_block<NB, L, true>(gr, tk, lane % 16 / L, lane % L, word, d);
     }
     if (again) key_exact<NB>(x, w, eps, cs, sn, gr, tk, lane, put, s_x);
