@@ -315,3 +315,28 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for g in got:
         assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+def test_experts_of_hidden_states_that_are_not_finite():
+    """Infinities and NaN among the hidden values, and the largest finite ones: each token still
+    goes to distinct experts, and its neighbours keep their values."""
+    import numpy as np
+    from tinygiant_b200.engine import MoEModel
+    m = MoEModel(256, 256, 8, 3, 1)
+    m.fill_synthetic(5)
+    rows = torch.randn(6, 256, generator=gen(1), device="cuda")
+    want = rows.clone()
+    m.moe_batched(0, want)
+    rows[0, 3], rows[0, 200] = float("inf"), float("inf")
+    rows[1, 3], rows[1, 200] = float("inf"), -float("inf")
+    rows[3, 7] = float("nan")
+    rows[4] = 3.4e38
+    got = rows.clone()
+    m.moe_batched(0, got)
+    assert torch.equal(got[[2, 5]], want[[2, 5]])
+    for row in rows:
+        m.moe_layer(0, row.clone())
+        idx, _, logits = m.last_routing(0)
+        order = sorted(range(8), key=lambda i: (np.where(np.isnan(logits), -np.inf, logits)[i], i), reverse=True)[:3]
+        assert sorted(idx) == sorted(order)
+    m.close()

@@ -9,6 +9,7 @@
 #include <stdint.h>
 
 #include "tg_layout.h"
+#include "tg_topk.h"
 
 namespace tg {
 
@@ -183,16 +184,11 @@ __device__ __forceinline__ Q8Lane quantize_lane(float v) {
 
 constexpr int MAX_TOPK = 16;
 
-// Top-k by rank: element i is selected when fewer than k elements beat it
-// (larger logit, or equal logit and larger id); its ascending position is k-1-rank.
+// Top-k by rank: element i is selected when fewer than k elements beat it (tg_topk.h); its
+// ascending position is k-1-rank.  Every sidx is written, as the ranks are all different.
 __device__ __forceinline__ void topk_softmax_block(const float* sl, int E, int k, int* sidx, float* sw) {
     for (int i = threadIdx.x; i < E; i += blockDim.x) {
-        float li = sl[i];
-        int rank = 0;
-        for (int j = 0; j < E; j++) {
-            float lj = sl[j];
-            rank += (lj > li) || (!(li > lj) && j > i);   // NaN too has its place: every sidx is written
-        }
+        const int rank = topk_rank(sl, E, i);
         if (rank < k) sidx[k - 1 - rank] = i;
     }
     __syncwarp();
