@@ -605,9 +605,9 @@ size_t tgx_kvq_page_bytes(int n_kv_heads, int head_dim, int page_tokens);
  * norm; rope_cos / rope_sin: fp32 [n_pos][head_dim / 2], or NULL for no rotation; the
  * position is the token's row, or positions[t] when given (device int32).  n_heads = 0 and
  * q = NULL: keys and values only.  q_out may be q (dense); it must not overlap k or v.
- * Two new tokens must not fall on the same page row.  All rows 4-element aligned (4 *
- * element size), strides multiples of 4.  Keys are computed in 64 bits, so codes are the
- * definition's; q in 32. */
+ * Two new tokens must not fall on the same page row.  All rows of q, k, v and q_out 4-element
+ * aligned (4 * element size), strides multiples of 4; norm weights, angles and positions aligned
+ * to their elements.  Codes of keys are those of 64-bit arithmetic; q in 32. */
 int tgx_kvq_append(const tgx_kvq_cache *cache, const tgx_kvq_batch *batch, int dtype, int n_tokens, const void *q,
                    long long q_stride, const void *k, long long k_stride, const void *v, long long v_stride,
                    int n_heads, const float *q_norm, const float *k_norm, float eps, const float *rope_cos,

@@ -401,6 +401,26 @@ def test_append_ties_zeros_and_values_out_of_range():
     assert torch.equal(s.pages, pages)
 
 
+@pytest.mark.parametrize("nh,nkv,hd,page", HEADS)
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_append_tables_at_any_element(nh, nkv, hd, page, off):
+    """Norm weights and angles as views into packed vectors, wherever they begin."""
+    s = Setup(APPENDS, nh, nkv, hd, page, BF16, seed=hd)
+    args = append_case(s, n_pos=70)
+    want = s.cache.append(s.batch, *args)
+    pages = s.pages.clone()
+
+    def packed(x):
+        flat = torch.full((x.numel() + 8,), 7.0, device="cuda")
+        view = flat[off:off + x.numel()].view(x.shape)
+        view.copy_(x)
+        assert view.data_ptr() % 16 == 4 * off
+        return view
+
+    s.pages.copy_(R.Cache(1, nkv, hd, page).pages(s.k, s.v))
+    got = s.cache.append(s.batch, *args[:3], *map(packed, args[3:]))
+    assert torch.equal(got, want) and torch.equal(s.pages, pages)
+
 @pytest.mark.parametrize("hd,gap", [(64, 4), (128, 8), (256, 16), (32, 2), (96, 6)])
 def test_append_keys_that_are_equal_in_32_bits_only(hd, gap):
     """Two rotated keys of one block that 32 bits round to the same magnitude: the larger of the

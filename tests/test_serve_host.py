@@ -82,6 +82,24 @@ def test_cache_refusals(clib):
         assert call() == (L.TG_ENODEV if clib.tg_device_count() == 0 else L.TG_EINVAL)
 
 
+
+def test_append_refuses_tables_off_their_elements(clib):
+    """Norm weights, angles and positions may begin at any element, but not inside one."""
+    buf = np.zeros(4096, np.uint8)
+    p = (buf.ctypes.data + 255) // 256 * 256
+    cache = L.TgxKvqCache(pages=p, n_pages=2, page_tokens=16, n_kv_heads=2, head_dim=64)
+    batch = L.TgxKvqBatch(n_seqs=1, max_pages=2, max_new=1, q_start=p, kv_lens=p, page_table=p, status=None)
+
+    def append(qn=p, kn=p, cos=p, sin=p, pos=p):
+        return clib.tgx_kvq_append(ctypes.byref(cache), ctypes.byref(batch), 0, 1, p, 256, p, 128, p, 128, 4, qn, kn, 1e-6,
+                                   cos, sin, 4, pos, p, None)
+
+    for name in ("qn", "kn", "cos", "sin", "pos"):
+        for off in (1, 2, 3):
+            refuse(clib, append(**{name: p + off}), "aligned to their elements")
+        assert append(**{name: p + 4}) == (L.TG_ENODEV if clib.tg_device_count() == 0 else L.TG_EINVAL)
+        assert "aligned" not in clib.tg_last_error().decode()
+
 def test_product_refusals(clib):
     buf = np.zeros(8192, np.uint8)
     p = (buf.ctypes.data + 255) // 256 * 256

@@ -52,6 +52,16 @@ __device__ __forceinline__ void load_row(float (&v)[N], const T* p) {
         for (int x = 0; x < W; x++) v[i + x] = to_f32(u.t[x]);
     }
 }
+// The same for norm weights and angles, which may begin at any element.
+template <int N>
+__device__ __forceinline__ void load_table(float (&v)[N], const float* p) {
+    if ((uintptr_t)p % (N % 4 == 0 ? 16 : 8) == 0) {
+        load_row(v, p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = p[i];
+    }
+}
 template <int N, typename T>
 __device__ __forceinline__ void store_row(T* p, const float (&v)[N]) {
     constexpr int W = N % 4 == 0 ? 4 : N % 2 == 0 ? 2 : 1;
@@ -86,7 +96,7 @@ __device__ __forceinline__ T norm_head(T (&x)[N], const float* w, float eps) {
     for (int o = 8; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const T mean = ss / (16 * N) + (T)eps, r = inv_sqrt(mean);
     float wn[N];
-    load_row(wn, w);
+    load_table(wn, w);
 #pragma unroll
     for (int i = 0; i < N; i++) x[i] = x[i] * r * (T)wn[i];
     return mean;
@@ -96,8 +106,8 @@ template <int N, typename T>
 __device__ __forceinline__ float rotate_head(T (&x)[N], const float* cs, const float* sn, int lane) {
     if (!cs) return 1.0f;
     float c[N], s[N], most = 1.0f;
-    load_row(c, cs);
-    load_row(s, sn);
+    load_table(c, cs);
+    load_table(s, sn);
 #pragma unroll
     for (int i = 0; i < N; i++) most = fmaxf(most, fmaxf(fabsf(c[i]), fabsf(s[i])));
 #pragma unroll
@@ -541,6 +551,9 @@ extern "C" int tgx_kvq_append(const tgx_kvq_cache* cache, const tgx_kvq_batch* b
     const size_t al = 4 * tg::elem_bytes(dtype);
     if (!tg::aligned(q, al) || !tg::aligned(k, al) || !tg::aligned(v, al) || !tg::aligned(q_out, al))
         return tg::serve_fail(TG_EINVAL, fn, "rows must be 4-element aligned");
+    if (!tg::aligned(q_norm, 4) || !tg::aligned(k_norm, 4) || !tg::aligned(rope_cos, 4) || !tg::aligned(rope_sin, 4) ||
+        !tg::aligned(positions, 4))
+        return tg::serve_fail(TG_EINVAL, fn, "norm weights, angles and positions must be aligned to their elements");
     if ((long long)n_tokens * (n_heads + 2 * cache->n_kv_heads) >= 0x7fff0000ll)
         return tg::serve_fail(TG_EINVAL, fn, "too many tokens for one call");
     tg::ServeDevice dev(fn, cache->pages);
