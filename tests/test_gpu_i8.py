@@ -186,3 +186,31 @@ def test_product_of_many_tiles(m, n, k, dtype):
             y.fill_(1)
             graph.replay()
             assert torch.equal(y, lin(x))
+
+
+def test_host_threads():
+    """Products of other tile widths from host threads, each on its own stream: no call disturbs
+    another's launch."""
+    import threading
+    from tinygiant_b200.int8 import Int8Linear
+    lin = Int8Linear.quantize(randn(1, 640, 512) * 0.05)
+    xs = [randn(2, 3, 512), randn(3, 200, 512)] * 2
+    want, wrong = [lin(x) for x in xs], []
+    torch.cuda.synchronize()
+
+    def work(x, y):
+        try:
+            stream = torch.cuda.Stream()
+            for _ in range(2000):
+                got = lin(x, stream=stream)
+            stream.synchronize()
+            assert torch.equal(got, y)
+        except Exception as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(xs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[0]

@@ -583,7 +583,8 @@ cudaError_t launch_mat(MatArgs g, const int8_t* x, const int8_t* w, int kp, cuda
     if (!row_map(&mw, w, g.N, kp, TM) || !row_map(&mx, x, g.M, kp, p.tn)) return cudaErrorInvalidValue;
     const int ring = p.stages * (TM * KB + p.tn * KB), part = p.splits > 1 ? p.tn * TM * 4 : 0;
     const int smem = (ring > part ? ring : part) + 1024;
-    cudaError_t e = cudaFuncSetAttribute(k_i8_mma<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // the same limit in every call: it is the kernel's, shared with other threads' calls of other sizes
+    cudaError_t e = cudaFuncSetAttribute(k_i8_mma<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.ctas);
