@@ -214,3 +214,16 @@ def test_host_threads():
     for t in threads:
         t.join()
     assert not wrong, wrong[0]
+
+
+def test_rows_of_zeros_under_weights_far_above_the_maximum():
+    """A weight times 127 / max |y| beyond fp32 meets values that are 0 or next to it."""
+    from tinygiant_b200.int8 import quantize_rows
+    for cols in (64, 50):
+        x = torch.zeros(3, cols, device="cuda")
+        w = torch.ones(cols, device="cuda")
+        w[5:9] = 1e10
+        x[0, 0], x[1, 0], x[2, 0] = 1e-28, 1e-28, -2e-29
+        x[1, 6], x[2, 7] = 3e-39, -1e-39     # products of 3e-29 and -1e-29
+        codes, _ = quantize_rows(x, w, 1e-5)
+        assert torch.equal(codes[:, :cols].double(), R.i8_rows(x, w, 1e-5)[0])

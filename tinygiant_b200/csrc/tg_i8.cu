@@ -66,7 +66,8 @@ __device__ __noinline__ int i8_code_exact(float x, float w, double top) { return
 // The codes of a piece, packed: rint(127 y / top) for y = x (or x * w, unrounded), |y| <= top, in
 // exact arithmetic.  Adding 1.5 * 2^23 rounds the fp32 quotient to a whole number, ties to even,
 // and leaves it in the low byte.  That quotient is off by less than 2^-15, so only what comes
-// that close to a border (2 in 10000, for a margin of 1e-4) needs the 64-bit one.
+// that close to a border (2 in 10000, for a margin of 1e-4) needs the 64-bit one; so does x next to
+// 0 under a w whose w * inv is beyond fp32, which leaves an infinity or NaN here.
 template <int V>
 __device__ __forceinline__ void i8_codes(uint32_t (&c)[V / 4], const float (&x)[V], const float (&w)[V], double top, float inv) {
     float t[V], far = 0.0f;
@@ -74,12 +75,12 @@ __device__ __forceinline__ void i8_codes(uint32_t (&c)[V / 4], const float (&x)[
     for (int i = 0; i < V; i++) {
         const float r = x[i] * (w[i] * inv);
         t[i] = __fadd_rn(r, 12582912.0f);
-        far = fmaxf(far, fabsf(r - __fsub_rn(t[i], 12582912.0f)));
+        far = max_nan(far, fabsf(r - __fsub_rn(t[i], 12582912.0f)));
     }
-    if (far >= 0.4999f) {
+    if (!(far < 0.4999f)) {
 #pragma unroll
         for (int i = 0; i < V; i++)
-            if (fabsf(x[i] * (w[i] * inv) - __fsub_rn(t[i], 12582912.0f)) >= 0.4999f)
+            if (!(fabsf(x[i] * (w[i] * inv) - __fsub_rn(t[i], 12582912.0f)) < 0.4999f))
                 t[i] = __int_as_float(i8_code_exact(x[i], w[i], top));
     }
 #pragma unroll
