@@ -521,3 +521,20 @@ def test_streams_and_two_graphs(new):
         torch.cuda.synchronize()
         assert torch.equal(outs[0], ref) and torch.equal(outs[1], ref)
     s.batch.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("new", [1, 12])
+def test_queries_that_are_not_finite(new, dtype):
+    """As for prompts: NaN out, 0 where there is no token to attend to, nothing at the neighbours."""
+    s = Setup([(new, 40 + new), (new, 300), (new, 0), (new, 90)], 8, 2, 64, 16, dtype, seed=12)
+    s.k[..., 3] = s.k[..., 3].abs() + 0.5
+    s.hk = R.held(s.k)
+    s.pages.copy_(R.Cache(1, 2, 64, 16).pages(s.k, s.v))
+    s.q[0, :, 3] = -float("inf")
+    s.q[new, :, 3] = float("nan")
+    s.q[2 * new, :, 3] = -float("inf")
+    got = s.cache.attention(s.batch, s.q)
+    assert torch.isnan(got[0]).all() and torch.isnan(got[new]).all() and (got[2 * new:3 * new] == 0).all()
+    rest = [t for t in range(s.T) if t not in (0, new) and not 2 * new <= t < 3 * new]
+    close(got[rest], *[x[rest] for x in s.expect()], 64, 300, dtype)

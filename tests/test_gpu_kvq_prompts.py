@@ -217,3 +217,25 @@ def test_waits_end_whatever_the_warps_pace(seqs):
     for _ in range(1500):
         bad += (s.cache.attention(s.batch, s.q) != want).sum()
     assert torch.isfinite(want.float()).all() and int(bad) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_queries_that_are_not_finite(dtype):
+    """An infinity or NaN in a query row makes its output NaN, whatever the scores' signs; a row
+    without a token to attend to is 0 all the same, and its neighbours keep their values."""
+    s = Setup([(200, 300), (200, 200), (200, 190), (200, 250)] * 2, 16, 2, 128, 64, dtype, seed=4)
+    s.k[..., 3] = s.k[..., 3].abs() + 0.5      # one sign in the dimension of the infinity
+    s.hk = R.held(s.k)
+    s.pages.copy_(R.Cache(1, s.nkv, s.hd, s.page).pages(s.k, s.v))
+    hit = torch.zeros(s.T, dtype=torch.bool)
+    for t, x in ((5, -float("inf")), (17, float("inf")), (199, float("nan")), (640, -float("inf")), (403, -float("inf"))):
+        s.q[t, :, 3] = x
+        hit[t] = True
+    got = s.cache.attention(s.batch, s.q)
+    none = torch.zeros(s.T, dtype=torch.bool)   # tokens in front of their sequence's first row
+    for b, (n, r) in enumerate(s.seqs):
+        none[s.start[b]:s.start[b] + max(0, n - r)] = True
+    assert hit[none].any() and (got[none.cuda()] == 0).all()
+    assert torch.isnan(got[(hit & ~none).cuda()]).all()
+    rest = ~(hit | none).cuda()
+    close(got[rest], *[x[rest] for x in s.expect()], 128, 300, dtype)

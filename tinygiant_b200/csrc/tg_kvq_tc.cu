@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             return (si.s0 + rho / a.R) * stride + (j * a.R + rho % a.R) * HD;
         };
         struct alignas(4 * sizeof(T)) Vec { T t[4]; };
-        float fac;
+        float fac, l;
         {
             unsigned top = 0;
             const int lr = lane / LPR, ld = lane % LPR * 4;   // the lane's row of those, and dimension
@@ -309,12 +309,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             }
             const int e = q_exp(top), half = e / 2;
             fac = a.scale * pow2(half) * pow2(e - half) * pow2(ex.x);
+            // an infinity's scores may all be -inf, which below is a row without a token to attend to
+            l = top >> 23 == 255 && lim > 0 ? __int_as_float(0x7fc00000) : 0.0f;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(q_full);
         }
         const uint32_t s_at = tmem + q * 128 + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t o_at = tmem + 256 + q * 128 + ((uint32_t)((warp & 3) * 32) << 16);
-        float m = -INFINITY, off = 0.0f, l = 0.0f;
+        float m = -INFINITY, off = 0.0f;
         bool good = true;
         for (int i = 0; i < tiles && good; i++) {
             good = __all_sync(0xffffffffu, mbar_wait(s_full(q, i), i >> 1 & 1, failed));
