@@ -546,6 +546,9 @@ int tgx_decode_token(tgx_attn *a, tgx_ctx *moe, float *x_dev, void *stream, int 
 #define TGX_F32 0
 #define TGX_BF16 1
 #define TGX_F16 2
+/* With TGX_BF16 or TGX_F16, where a function says so: the rows x are fp32, each element rounded to
+ * the 16-bit type as it is read.  A finite one beyond that type's range stays as it is. */
+#define TGX_FROM_F32 16
 
 /* One layer's keys and values of many sequences, in pages of page_tokens tokens (a
  * multiple of 16, at most 1024): pages[n_pages] of tgx_kvq_page_bytes bytes each, 16-byte
@@ -638,7 +641,7 @@ int tgx_kvq_attention(const tgx_kvq_cache *cache, const tgx_kvq_batch *batch, in
  * to even), scale max |y| / 127, with norm_w times the RMSNorm factor 1 / sqrt(mean x^2 +
  * eps): codes * scale stands for the row, or for its RMSNorm.  A row with a value that is not
  * finite gets scale NaN and codes 0; a zero row scale 0.  x: rows x_stride elements apart.
- * codes 16-byte aligned. */
+ * codes 16-byte aligned.  dtype may have TGX_FROM_F32. */
 size_t tgx_i8_row_bytes(int cols);
 int tgx_i8_quantize_rows(int dtype, const void *x, long long x_stride, int rows, int cols, const float *norm_w,
                          float eps, int8_t *codes, float *scales, void *stream);
@@ -646,8 +649,9 @@ int tgx_i8_quantize_rows(int dtype, const void *x, long long x_stride, int rows,
 /* out[m][n] = sum_k a[m][k] w[n][k] * (sa[m] * sw[n]) (+ residual[m][n]): a, sa the rows of x
  * quantised as above (norm_w NULL or the RMSNorm in front), w, sw int8 rows and scales of
  * tgx_i8_quantize_rows (16-byte aligned).  The integer sum is exact (k <= 131072); the rest
- * fp32, rounded once to `dtype`.  residual may be out.  scratch: tgx_i8_matmul_scratch_bytes
- * bytes, 256-byte aligned, no contents assumed or kept; calls sharing it must be ordered. */
+ * fp32, rounded once to `dtype`.  residual may be out.  dtype may have TGX_FROM_F32: x is fp32, out
+ * and residual of the 16-bit type.  scratch: tgx_i8_matmul_scratch_bytes bytes, 256-byte aligned,
+ * no contents assumed or kept; calls sharing it must be ordered. */
 size_t tgx_i8_matmul_scratch_bytes(int m, int n, int k);
 int tgx_i8_matmul(int dtype, const void *x, long long x_stride, int m, int k, const float *norm_w, float eps,
                   const int8_t *w_codes, const float *w_scales, int n, const void *residual, long long res_stride,

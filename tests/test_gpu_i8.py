@@ -227,3 +227,41 @@ def test_rows_of_zeros_under_weights_far_above_the_maximum():
         x[1, 6], x[2, 7] = 3e-39, -1e-39     # products of 3e-29 and -1e-29
         codes, _ = quantize_rows(x, w, 1e-5)
         assert torch.equal(codes[:, :cols].double(), R.i8_rows(x, w, 1e-5)[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("m,n,k", [(1, 300, 2048), (3, 129, 47), (70, 257, 333), (2100, 64, 400)])
+def test_fp32_rows_as_a_16_bit_type(m, n, k, dtype):
+    """The same bits as from x.to(dtype), strided rows included; finite values beyond the type's
+    range, which would become infinities there, count as they are."""
+    from tinygiant_b200.int8 import Int8Linear
+    lin = Int8Linear.quantize(randn(1, n, k) * 0.05)
+    wide = randn(2, m, k + 9) * 10.0 ** torch.randint(-6, 3, (m, 1), generator=torch.Generator().manual_seed(k)).cuda()
+    norm, res = 1 + 0.2 * randn(3, k), randn(4, m, n).to(dtype)
+    for x in (wide[:, 5:5 + k], wide[:, 5:5 + k].contiguous()):
+        y = x.to(dtype)
+        assert torch.equal(lin(x, dtype=dtype), lin(y))
+        assert torch.equal(lin(x, norm=norm, residual=res, dtype=dtype), lin(y, norm=norm, residual=res))
+    big = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).cuda()
+    big[:, ::7] *= 1e6 if dtype == F16 else 1e20
+    if dtype == BF16:
+        big[:, 0] = 3.4e38                        # rounds to an infinity in bfloat16
+    rounded = torch.where(torch.isfinite(big.to(dtype)), big.to(dtype).float(), big)
+    assert torch.equal(lin(big, dtype=dtype), lin(rounded).to(dtype))
+    if dtype == F16:   # squares of 3e38 are beyond fp32's sums
+        got, want = lin(big, norm=norm, dtype=dtype).double(), lin(rounded, norm=norm).double()
+        # sums of squares in another order, and the type's rounding
+        assert ((got - want).abs() <= (k * 2.0 ** -24 + 1.001 * 2.0 ** -11) * want.abs() + 2.0 ** -25).all()
+
+
+
+def test_refuses_other_types_of_rows():
+    from tinygiant_b200.int8 import Int8Linear
+    lin = Int8Linear.quantize(randn(1, 8, 32))
+    x = randn(2, 3, 32)
+    for bad in (dict(x=x.half(), dtype=BF16), dict(x=x.half(), dtype=F32), dict(x=x, dtype=torch.float64), dict(x=x.double())):
+        with pytest.raises(TypeError):
+            lin(**bad)
+    for bad in (dict(out=torch.empty(3, 8, device="cuda")), dict(residual=torch.zeros(3, 8, device="cuda"))):
+        with pytest.raises(ValueError):
+            lin(x, dtype=BF16, **bad)

@@ -340,3 +340,18 @@ def test_experts_of_hidden_states_that_are_not_finite():
         order = sorted(range(8), key=lambda i: (np.where(np.isnan(logits), -np.inf, logits)[i], i), reverse=True)[:3]
         assert sorted(idx) == sorted(order)
     m.close()
+
+
+def test_hidden_values_beyond_the_16_bit_types(dtype=F16):
+    """A hidden state with values that fp16 does not reach: the norm brings them back."""
+    a, _ = build(dtype)
+    b, _ = build(F32)
+    X = torch.randn(9, EMB, generator=gen(3), device="cuda")
+    X[2, 5], X[4, 7], X[4, 100] = 1e5, -3e6, 2e6
+    X[6] *= 1e5
+    want = b.layer(0, batch_of([(9, 9)]), X.clone())
+    got = a.layer(0, batch_of([(9, 9)]), X.clone())
+    assert torch.isfinite(got).all()
+    # the layer's own term, to what 8-bit codes and 4-bit rows that fall on the other side of a border may cost
+    d, size = (got - want).norm(dim=1), (want - X).norm(dim=1)
+    assert (d <= 0.2 * size).all(), (d / size).tolist()

@@ -124,6 +124,27 @@ def test_product_refusals(clib):
         refuse(clib, rows(**kw), text)
 
 
+
+def test_types_of_fp32_rows(clib):
+    """TGX_FROM_F32 goes with a 16-bit type, with x aligned as fp32 and out as the type."""
+    buf = np.zeros(8192, np.uint8)
+    p = (buf.ctypes.data + 255) // 256 * 256
+    none = L.TG_ENODEV if clib.tg_device_count() == 0 else L.TG_EINVAL
+
+    def mat(dtype, x=p, out=p):
+        return clib.tgx_i8_matmul(dtype, x, 32, 2, 32, None, 0.0, p, p, 8, None, 0, out, 8, p, 4096, None)
+
+    def rows(dtype, x=p):
+        return clib.tgx_i8_quantize_rows(dtype, x, 32, 2, 32, None, 0.0, p, p, None)
+
+    for call in (mat, rows):
+        for bad in (L.TGX_FROM_F32 | L.TGX_F32, L.TGX_FROM_F32 | 3, 32 | L.TGX_BF16, -1):
+            refuse(clib, call(bad), "dtype")
+        for good in (L.TGX_BF16, L.TGX_F16):
+            assert call(good | L.TGX_FROM_F32) == none and "dtype" not in clib.tg_last_error().decode()
+            refuse(clib, call(good | L.TGX_FROM_F32, x=p + 2), "elements")
+    assert mat(L.TGX_F16 | L.TGX_FROM_F32, out=p + 2) == none and "elements" not in clib.tg_last_error().decode()
+
 def test_python_refusals():
     from tinygiant_b200.int8 import Int8Linear, quantize_rows
     from tinygiant_b200.paged import PagedBatch, PagedKV4, dtype_code

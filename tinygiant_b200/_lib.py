@@ -43,6 +43,7 @@ TGX_MULTI = 2
 TGX_F32 = 0
 TGX_BF16 = 1
 TGX_F16 = 2
+TGX_FROM_F32 = 16
 
 TGX_KVQ_BAD_PAGE = 1
 TGX_KVQ_BAD_LENGTH = 2

@@ -29,18 +29,43 @@ struct QuantArgs {
     float* scales;
 };
 
-// 16 bytes of x as floats, and their norm weights: in one piece (ALL), or element by element
-// with zeros behind the row.
-template <bool ALL, int V, typename T>
-__device__ __forceinline__ void load_piece(float (&v)[V], const T* x, int at, int cols) {
+// A row's type: its elements, how many make a piece, and an element's value.  fp32 taken as a 16-bit
+// type (TGX_FROM_F32) is rounded to it, unless it is finite and the rounding is not; its pieces are
+// the 16-bit type's, so that both give the same sums.
+template <int DT> struct Row {
+    using T = typename Elem<DT & ~TGX_FROM_F32>::T;
+    static constexpr int V = 16 / sizeof(T);
+    __device__ __forceinline__ static float value(T x) { return to_f32(x); }
+};
+template <int DT> struct Rounded {
+    using T = float;
+    static constexpr int V = 8;
+    __device__ __forceinline__ static float value(float x) {
+        typename Elem<DT>::T r;
+        from_f32(x, r);
+        return fabsf(to_f32(r)) <= 3.4028235e38f ? to_f32(r) : x;
+    }
+};
+template <> struct Row<TGX_BF16 | TGX_FROM_F32> : Rounded<TGX_BF16> {};
+template <> struct Row<TGX_F16 | TGX_FROM_F32> : Rounded<TGX_F16> {};
+
+// A piece of x as floats, and its norm weights: in 16-byte loads (ALL), or element by element with
+// zeros behind the row.
+template <int DT, bool ALL, int V>
+__device__ __forceinline__ void load_piece(float (&v)[V], const typename Row<DT>::T* x, int at, int cols) {
+    using T = typename Row<DT>::T;
     if constexpr (ALL) {
-        const uint4 u = *reinterpret_cast<const uint4*>(x + at);
-        const T* t = reinterpret_cast<const T*>(&u);
+        constexpr int N = 16 / sizeof(T);
 #pragma unroll
-        for (int i = 0; i < V; i++) v[i] = to_f32(t[i]);
+        for (int i = 0; i < V; i += N) {
+            const uint4 u = *reinterpret_cast<const uint4*>(x + at + i);
+            const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int y = 0; y < N; y++) v[i + y] = Row<DT>::value(t[y]);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < V; i++) v[i] = at + i < cols ? to_f32(x[at + i]) : 0.0f;
+        for (int i = 0; i < V; i++) v[i] = at + i < cols ? Row<DT>::value(x[at + i]) : 0.0f;
     }
 }
 template <bool NORM, bool ALL, int V>
@@ -99,8 +124,8 @@ __device__ __forceinline__ void i8_codes(uint32_t (&c)[V / 4], const float (&x)[
 // (G = 1).  For few rows, by latency: a CTA each (G = 8).
 template <int DT, bool NORM, bool VEC, int G>
 __global__ void __launch_bounds__(256, 4) k_i8_rows(QuantArgs a) {
-    using T = typename Elem<DT>::T;
-    constexpr int V = 16 / sizeof(T), NT = 32 * G;
+    using T = typename Row<DT>::T;
+    constexpr int V = Row<DT>::V, NT = 32 * G;
     static_assert(G == 1 || G == 8, "a warp or a CTA of 256 threads per row");
     __shared__ float s_hi[8], s_ss[8];
     __shared__ double s_top[8];
@@ -119,13 +144,13 @@ __global__ void __launch_bounds__(256, 4) k_i8_rows(QuantArgs a) {
         int i = 0, c = tid;
 #pragma unroll 2
         for (; c < whole; c += NT, i++) {
-            load_piece<true>(v, x, c * V, a.cols);
+            load_piece<DT, true>(v, x, c * V, a.cols);
             load_norm<NORM, true>(w, a.norm, c * V, a.cols);
             f(v, w, c * V, min(i, 31));
         }
 #pragma unroll 1
         for (; c < pieces; c += NT, i++) {
-            load_piece<false>(v, x, c * V, a.cols);
+            load_piece<DT, false>(v, x, c * V, a.cols);
             load_norm<NORM, false>(w, a.norm, c * V, a.cols);
             f(v, w, c * V, min(i, 31));
         }
@@ -174,7 +199,7 @@ __global__ void __launch_bounds__(256, 4) k_i8_rows(QuantArgs a) {
             for (uint32_t left = where; left; left &= left - 1) {
                 const int c = (tid + (__ffs(left) - 1) * NT) * V;
                 float v[V], w[V];
-                load_piece<false>(v, x, c, a.cols);
+                load_piece<DT, false>(v, x, c, a.cols);
                 load_norm<NORM, false>(w, a.norm, c, a.cols);
                 largest(v, w);
             }
@@ -606,7 +631,7 @@ cudaError_t launch_mat(MatArgs g, const int8_t* x, const int8_t* w, int kp, cuda
 
 template <int DT>
 cudaError_t launch_rows(const QuantArgs& a, cudaStream_t s) {
-    constexpr int E = DT == TGX_F32 ? 4 : 2;
+    constexpr int E = sizeof(typename Row<DT>::T);
     const bool vec = ((uintptr_t)a.x | (uintptr_t)(a.xs * E) | (uintptr_t)a.norm) % 16 == 0;
     // a warp per row once that fills the device (148 SMs of 24 such warps) and rows are no longer
     // than a few thousand: 8100 x 2048 bf16 took 41 us a CTA each
@@ -625,9 +650,20 @@ cudaError_t launch_rows(const QuantArgs& a, cudaStream_t s) {
 }
 
 cudaError_t launch_rows(int dtype, const QuantArgs& a, cudaStream_t s) {
-    return dtype == TGX_F32 ? launch_rows<TGX_F32>(a, s)
-                            : dtype == TGX_BF16 ? launch_rows<TGX_BF16>(a, s) : launch_rows<TGX_F16>(a, s);
+    switch (dtype) {
+        case TGX_F32: return launch_rows<TGX_F32>(a, s);
+        case TGX_BF16: return launch_rows<TGX_BF16>(a, s);
+        case TGX_F16: return launch_rows<TGX_F16>(a, s);
+        case TGX_BF16 | TGX_FROM_F32: return launch_rows<TGX_BF16 | TGX_FROM_F32>(a, s);
+        default: return launch_rows<TGX_F16 | TGX_FROM_F32>(a, s);
+    }
 }
+
+// Whether the rows may be of that type, and the bytes of an element.
+bool row_type(int dtype) {
+    return (dtype >= TGX_F32 && dtype <= TGX_F16) || dtype == (TGX_BF16 | TGX_FROM_F32) || dtype == (TGX_F16 | TGX_FROM_F32);
+}
+int row_elem(int dtype) { return dtype & TGX_FROM_F32 ? 4 : elem_bytes(dtype); }
 
 size_t r256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -641,10 +677,10 @@ extern "C" int tgx_i8_quantize_rows(int dtype, const void* x, long long x_stride
                                     const float* norm_w, float eps, int8_t* codes, float* scales, void* stream) {
     const char* fn = "tgx_i8_quantize_rows";
     if (!x || !codes || !scales) return tg::serve_fail(TG_EINVAL, fn, "null pointer");
-    if (dtype < TGX_F32 || dtype > TGX_F16) return tg::serve_fail(TG_EINVAL, fn, "unknown dtype");
+    if (!tg::row_type(dtype)) return tg::serve_fail(TG_EINVAL, fn, "unknown dtype");
     if (rows < 0 || !tgx_i8_row_bytes(cols) || x_stride < cols || !(eps >= 0.0f))
         return tg::serve_fail(TG_EINVAL, fn, "bad rows, cols (1 .. 131072), stride or eps");
-    if (!tg::aligned(codes, 16) || !tg::aligned(x, tg::elem_bytes(dtype)))
+    if (!tg::aligned(codes, 16) || !tg::aligned(x, tg::row_elem(dtype)))
         return tg::serve_fail(TG_EINVAL, fn, "codes must be 16-byte aligned, x to its elements");
     tg::ServeDevice dev(fn, x);
     if (dev.rc != TG_OK || rows == 0) return dev.rc;
@@ -664,12 +700,13 @@ extern "C" int tgx_i8_matmul(int dtype, const void* x, long long x_stride, int m
                              void* stream) {
     const char* fn = "tgx_i8_matmul";
     if (!x || !w_codes || !w_scales || !out || !scratch) return tg::serve_fail(TG_EINVAL, fn, "null pointer");
-    if (dtype < TGX_F32 || dtype > TGX_F16) return tg::serve_fail(TG_EINVAL, fn, "unknown dtype");
+    if (!tg::row_type(dtype)) return tg::serve_fail(TG_EINVAL, fn, "unknown dtype");
     if (m < 0 || n <= 0 || !tgx_i8_row_bytes(k) || x_stride < k || out_stride < n || (residual && res_stride < n) ||
         !(eps >= 0.0f))
         return tg::serve_fail(TG_EINVAL, fn, "bad m, n, k (1 .. 131072), stride or eps");
-    const size_t e1 = tg::elem_bytes(dtype);
-    if (!tg::aligned(w_codes, 16) || !tg::aligned(x, e1) || !tg::aligned(out, e1) || !tg::aligned(residual, e1))
+    const int type = dtype & ~TGX_FROM_F32;   // of out and residual
+    const size_t e1 = tg::elem_bytes(type);
+    if (!tg::aligned(w_codes, 16) || !tg::aligned(x, tg::row_elem(dtype)) || !tg::aligned(out, e1) || !tg::aligned(residual, e1))
         return tg::serve_fail(TG_EINVAL, fn, "w_codes must be 16-byte aligned, x, residual and out to their elements");
     if (!tg::aligned(scratch, 256) || scratch_bytes < tgx_i8_matmul_scratch_bytes(m, n, k))
         return tg::serve_fail(TG_EINVAL, fn, "scratch must be 256-byte aligned, of tgx_i8_matmul_scratch_bytes");
@@ -683,8 +720,8 @@ extern "C" int tgx_i8_matmul(int dtype, const void* x, long long x_stride, int m
     cudaError_t e = tg::launch_rows(dtype, qa, s);
     if (e != cudaSuccess) return tg::serve_fail(TG_ECUDA, fn, cudaGetErrorString(e));
     tg::MatArgs g{scales, w_scales, m, n, residual, res_stride, out, out_stride, 0, 0, 0, 0};
-    e = dtype == TGX_F32    ? tg::launch_mat<TGX_F32>(g, codes, w_codes, kp, s)
-        : dtype == TGX_BF16 ? tg::launch_mat<TGX_BF16>(g, codes, w_codes, kp, s)
-                            : tg::launch_mat<TGX_F16>(g, codes, w_codes, kp, s);
+    e = type == TGX_F32    ? tg::launch_mat<TGX_F32>(g, codes, w_codes, kp, s)
+        : type == TGX_BF16 ? tg::launch_mat<TGX_BF16>(g, codes, w_codes, kp, s)
+                           : tg::launch_mat<TGX_F16>(g, codes, w_codes, kp, s);
     return e == cudaSuccess ? TG_OK : tg::serve_fail(TG_ECUDA, fn, cudaGetErrorString(e));
 }

@@ -10,8 +10,8 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import check, get_lib
-from .paged import dtype_code, on_stream, stream_handle
+from ._lib import TGX_FROM_F32, check, get_lib
+from .paged import DTYPES, dtype_code, on_stream, stream_handle
 
 
 def _matrix(t, cols, device, name):
@@ -74,32 +74,39 @@ class Int8Linear:
         """From float32, bfloat16 or float16 weights [N][K] on the device."""
         return cls(*quantize_rows(weight, stream=stream), weight.shape[1])
 
-    def __call__(self, x, out=None, norm=None, eps: float = 1e-6, residual=None, stream=None):
+    def __call__(self, x, out=None, norm=None, eps: float = 1e-6, residual=None, stream=None, dtype=None):
         """x [M][K] W^T (+ residual) -> out [M][N] of x's type, x quantised per row, behind its
-        RMSNorm when `norm` is given.  out may be residual."""
+        RMSNorm when `norm` is given.  out may be residual.  dtype: a 16-bit type for out and
+        residual with a float32 x, which is rounded to it as x.to(dtype) would, but keeps finite
+        values beyond its range."""
         if stream is not None:
             with on_stream(stream, self.device):
-                return self(x, out, norm, eps, residual)
+                return self(x, out, norm, eps, residual, None, dtype)
         dev, k, n = self.device, self.in_features, self.out_features
+        code, dtype = dtype_code(x), dtype or x.dtype
+        if dtype != x.dtype:
+            if x.dtype != torch.float32 or dtype not in DTYPES:
+                raise TypeError(f"no product of {x.dtype} rows to {dtype}")
+            code = DTYPES[dtype] | TGX_FROM_F32
         px, sx = _matrix(x, k, dev, "x")
         m = x.shape[0]
         if out is None:
-            out = x.new_empty((m, n))
+            out = x.new_empty((m, n), dtype=dtype)
             po, so = out.data_ptr(), n
         else:
             po, so = _matrix(out, n, dev, "out")
-            if out.dtype != x.dtype or out.shape[0] != m:
-                raise ValueError("out: expected x's type and rows")
+            if out.dtype != dtype or out.shape[0] != m:
+                raise ValueError(f"out: expected {m} rows of {dtype}")
         pr, sr = None, 0
         if residual is not None:
             pr, sr = _matrix(residual, n, dev, "residual")
-            if residual.dtype != x.dtype or residual.shape[0] != m:
-                raise ValueError("residual: expected x's type and rows")
+            if residual.dtype != dtype or residual.shape[0] != m:
+                raise ValueError(f"residual: expected {m} rows of {dtype}")
         if not m:
             return out
         size = self.lib.tgx_i8_matmul_scratch_bytes(m, n, k)
         scratch = self.codes.new_empty(size)
-        check(self.lib.tgx_i8_matmul(dtype_code(x), px, sx, m, k, _norm(norm, k, dev), eps, self.codes.data_ptr(),
+        check(self.lib.tgx_i8_matmul(code, px, sx, m, k, _norm(norm, k, dev), eps, self.codes.data_ptr(),
                                      self.scales.data_ptr(), n, pr, sr, po, so, scratch.data_ptr(), size,
                                      stream_handle(dev)), self.lib)
         return out

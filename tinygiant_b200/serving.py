@@ -22,7 +22,9 @@ class BatchedAttention:
 
     One page table serves every layer: page p of a sequence is page p of each layer's cache.
     dtype is the type between the two projections of a layer: float32, or bfloat16 / float16,
-    whose attention over long prompts runs on the 16-bit tensor cores."""
+    whose attention over long prompts runs on the 16-bit tensor cores.  X's elements count as
+    rounded to it in front of the norm (those beyond its range stay as they are), and the output
+    projection is rounded to it before it is added to X."""
 
     def __init__(self, embed=C.EMBED_DIM, n_heads=C.N_HEADS, n_kv_heads=C.N_KV_HEADS, head_dim=C.HEAD_DIM,
                  n_layers=C.N_LAYERS, n_pages=1024, page_tokens=64, max_pos=4096, dtype=torch.float32, device=0,
@@ -80,7 +82,7 @@ class BatchedAttention:
             raise ValueError(f"layer {layer} has no weights")
         wqkv, wo, attn_norm, q_norm, k_norm = self.layers[layer]
         cache, qd, kvd = self.caches[layer], self.n_heads * self.head_dim, self.n_kv_heads * self.head_dim
-        q, k, v = wqkv(X.to(self.dtype), norm=attn_norm, eps=self.eps).split((qd, kvd, kvd), 1)
+        q, k, v = wqkv(X, norm=attn_norm, eps=self.eps, dtype=self.dtype).split((qd, kvd, kvd), 1)
         # rows behind the batch's last token are in nobody's sequence: zeros there leave X's as they are
         o = X.new_zeros((X.shape[0], qd), dtype=self.dtype)
         cache.append(batch, q, k, v, self.cos, self.sin, q_norm, k_norm, self.eps, q_out=o)
