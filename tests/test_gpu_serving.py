@@ -355,3 +355,13 @@ def test_hidden_values_beyond_the_16_bit_types(dtype=F16):
     # the layer's own term, to what 8-bit codes and 4-bit rows that fall on the other side of a border may cost
     d, size = (got - want).norm(dim=1), (want - X).norm(dim=1)
     assert (d <= 0.2 * size).all(), (d / size).tolist()
+
+
+def test_device_without_an_index():
+    from tinygiant_b200.serving import BatchedAttention
+    a = BatchedAttention(64, 2, 1, 64, 1, 4, device="cuda")
+    a.fill_synthetic(1)
+    X = torch.randn(2, 64, device="cuda")
+    b = BatchedAttention(64, 2, 1, 64, 1, 4, device=0)
+    b.fill_synthetic(1)
+    assert torch.equal(a.layer(0, batch_of([(2, 2)], width=4), X.clone()), b.layer(0, batch_of([(2, 2)], width=4), X.clone()))

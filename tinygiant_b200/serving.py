@@ -36,6 +36,8 @@ class BatchedAttention:
         self.embed, self.n_heads, self.n_kv_heads, self.head_dim = embed, n_heads, n_kv_heads, head_dim
         self.n_layers, self.dtype, self.eps = n_layers, dtype, float(eps)
         self.device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self.caches = [PagedKV4(n_kv_heads, head_dim, page_tokens, n_pages, device=self.device) for _ in range(n_layers)]
         self.layers = [None] * n_layers
         self.cos, self.sin = (torch.from_numpy(a).to(self.device) for a in rope_cache(max_pos, head_dim))
