@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     constexpr int HD = 32 * NB, ATOM = QT * 128;               // bytes of 64 dimensions of 128 rows
     constexpr int Q_BYTES = NB / 2 * ATOM, SLOT = 4096 * NB, K_ATOM = TK * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t s_bars[13 + 2 * SLOTS];
+    __shared__ __align__(8) uint64_t s_bars[15 + 2 * SLOTS];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
     __shared__ __align__(4) uint8_t s_valid[8][TK / 16];   // [tile % 8]: whether its granules exist
@@ -221,6 +221,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     auto full = [&](int slot) { return bars + 88 + 8 * slot; };
     auto empty = [&](int slot) { return bars + 88 + 8 * SLOTS + 8 * slot; };
     auto o_done = [&](int q) { return bars + 88 + 16 * SLOTS + 8 * q; };   // O's last sum
+    auto at_rest = [&](int q) { return bars + 104 + 16 * SLOTS + 8 * q; };  // all that was issued, where a wait failed
 
     const int item = blockIdx.x / a.c.nkv, j = blockIdx.x % a.c.nkv;   // the longest first
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
         for (int i = 1; i < 7; i++) mbar_init(&s_bars[i], 1);
         for (int i = 7; i < 11; i++) mbar_init(&s_bars[i], QT);
         for (int i = 0; i < SLOTS; i++) mbar_init(&s_bars[11 + i], 16 * DW), mbar_init(&s_bars[11 + SLOTS + i], 2);
-        for (int i = 0; i < 2; i++) mbar_init(&s_bars[11 + 2 * SLOTS + i], 1);
+        for (int i = 0; i < 4; i++) mbar_init(&s_bars[11 + 2 * SLOTS + i], 1);
         s_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;");
     }
@@ -569,9 +570,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
                 step(vslot, vphase);
             }
             if (!good) {   // what is under way ends before the TMEM is freed: one more commit behind it all
-                if (elect_one()) commit(q_full);
+                if (elect_one()) commit(at_rest(q));
                 const long long t0 = clock64();
-                while (!mbar_try(q_full, 1) && clock64() - t0 < WAIT_CYCLES / 16) {
+                while (!mbar_try(at_rest(q), 0) && clock64() - t0 < WAIT_CYCLES) {
                 }
             }
         }
