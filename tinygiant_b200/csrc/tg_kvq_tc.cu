@@ -208,14 +208,16 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
     constexpr int HD = 32 * NB, ATOM = QT * 128;               // bytes of 64 dimensions of 128 rows
     constexpr int Q_BYTES = NB / 2 * ATOM, SLOT = 4096 * NB, K_ATOM = TK * 128;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t s_bars[15 + 2 * SLOTS];
+    __shared__ __align__(8) uint64_t s_bars[17 + 2 * SLOTS];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed;
     __shared__ __align__(4) uint8_t s_valid[8][TK / 16];   // [tile % 8]: whether its granules exist
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t bars = saddr_kept(s_bars), q_full = bars;
-    auto pv_done = [&](int q) { return bars + 8 + 8 * q; };
+    // of tile i, one for the even and one for the odd: a parity tells neighbouring phases apart only, and
+    // nothing says that tile i - 2's arrival is there before that of the scores of tile i
+    auto pv_done = [&](int q, int i) { return bars + 8 + 8 * q + (i & 1) * (112 + 16 * SLOTS); };
     auto s_full = [&](int q, int i) { return bars + 24 + 16 * q + 8 * (i & 1); };    // of tile i
     auto p_ready = [&](int q, int i) { return bars + 56 + 16 * q + 8 * (i & 1); };
     auto full = [&](int slot) { return bars + 88 + 8 * slot; };
@@ -242,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
         for (int i = 1; i < 7; i++) mbar_init(&s_bars[i], 1);
         for (int i = 7; i < 11; i++) mbar_init(&s_bars[i], QT);
         for (int i = 0; i < SLOTS; i++) mbar_init(&s_bars[11 + i], 16 * DW), mbar_init(&s_bars[11 + SLOTS + i], 2);
-        for (int i = 0; i < 4; i++) mbar_init(&s_bars[11 + 2 * SLOTS + i], 1);
+        for (int i = 0; i < 6; i++) mbar_init(&s_bars[11 + 2 * SLOTS + i], 1);
         s_failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;");
     }
@@ -346,7 +348,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
                 off = m == -INFINITY ? 0.0f : P_EXP - m;
                 l *= f;
                 if (i) {
-                    good = __all_sync(0xffffffffu, mbar_wait(pv_done(q), (i - 1) & 1, failed));   // O is at rest
+                    good = __all_sync(0xffffffffu, mbar_wait(pv_done(q, i - 1), (i - 1) >> 1 & 1, failed));   // O is at rest
                     if (!good) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -376,8 +378,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             mbar_arrive(p_ready(q, i));
         }
-        // a barrier of its own: a parity of pv_done's tells neighbouring phases apart, and this warp may be
-        // two ahead of it (another's p of the tile in front is missing) or two behind
+        // a barrier of its own, which completes once: no phase to take for another
         if (good && tiles) good = __all_sync(0xffffffffu, mbar_wait(o_done(q), 0, failed));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const float inv = !good ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
@@ -535,7 +536,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
                 if (elect_one()) {
 #pragma unroll
                     for (int s = 0; s < TK / 16; s++) mma_f16_ts(d, x + 8 * s, y + (s * 32 >> 4), IDESC_O, i > 0 || s > 0);
-                    commit(pv_done(q));
+                    commit(pv_done(q, i));
                     if (i + 1 == tiles) commit(o_done(q));
                     commit(empty(slot));
                 }
