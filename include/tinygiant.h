@@ -582,7 +582,8 @@ typedef struct {
  * the contents do not fit: a page id outside the cache or a length beyond the table (such
  * rows are neither written nor attended to), a new token with a negative row or a rope
  * position outside the tables (not written, its outputs 0), more new tokens than max_new
- * (not attended: left as they are). */
+ * (those behind are not attended: left as they are) or than the call's rows, or starts that go
+ * back (none of the sequence's are). */
 typedef struct {
     int n_seqs;
     int max_pages;

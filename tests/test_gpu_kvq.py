@@ -538,3 +538,18 @@ def test_queries_that_are_not_finite(new, dtype):
     assert torch.isnan(got[0]).all() and torch.isnan(got[new]).all() and (got[2 * new:3 * new] == 0).all()
     rest = [t for t in range(s.T) if t not in (0, new) and not 2 * new <= t < 3 * new]
     close(got[rest], *[x[rest] for x in s.expect()], 64, 300, dtype)
+
+
+@pytest.mark.parametrize("start", [[0, 2, 9], [0, 5, 4], [-1, 2, 4], [0, 2, 2 ** 31 - 1]])
+def test_starts_that_do_not_fit_are_reported(start):
+    """A sequence whose new tokens are not the step's rows is left out, and check() says so."""
+    s = Setup([(2, 50), (2, 60)], 4, 2, 64, 16, F32, seed=8)
+    want = s.cache.attention(s.batch, s.q)
+    s.batch.check()
+    s.batch.q_start.copy_(torch.tensor(start, dtype=torch.int32))
+    dst = torch.full_like(s.q, 3.0)
+    s.cache.attention(s.batch, s.q, out=dst)
+    if start[:2] == [0, 2]:
+        assert torch.equal(dst[:2], want[:2]) and (dst[2:] == 3).all()
+    with pytest.raises(RuntimeError, match="starts that go back"):
+        s.batch.check()

@@ -146,7 +146,8 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
             mine += n;
             grans += n * s.grans;
             if (w == 0 && (long long)a.b.kv_lens[b] > (long long)a.b.max_pages * a.c.pt) kvq_flag(a.b, TGX_KVQ_BAD_LENGTH);
-            if (w == 0 && (long long)a.b.q_start[b + 1] - a.b.q_start[b] > a.b.max_new) kvq_flag(a.b, TGX_KVQ_BAD_NEW);
+            const int s0 = a.b.q_start[b], s1 = a.b.q_start[b + 1];
+            if (w == 0 && (s0 < 0 || s1 < s0 || s1 > a.T || s1 - s0 > a.b.max_new)) kvq_flag(a.b, TGX_KVQ_BAD_NEW);
         }
     }
     if (tid < 2) a.heads[((size_t)w * 2 + tid) * 4] = SLOT_NONE;   // no slots yet

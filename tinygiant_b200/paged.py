@@ -104,7 +104,7 @@ class PagedBatch:
             said = [text for bit, text in ((TGX_KVQ_BAD_PAGE, "a page id outside the cache"),
                                            (TGX_KVQ_BAD_LENGTH, "a length beyond the page table or fewer rows than new tokens"),
                                            (TGX_KVQ_BAD_POSITION, "a position outside the rope tables"),
-                                           (TGX_KVQ_BAD_NEW, "more new tokens than max_new")) if bits & bit]
+                                           (TGX_KVQ_BAD_NEW, "more new tokens than max_new or the step's rows, or starts that go back")) if bits & bit]
             raise RuntimeError("paged cache: " + ", ".join(said))
 
 
