@@ -553,3 +553,22 @@ def test_starts_that_do_not_fit_are_reported(start):
         assert torch.equal(dst[:2], want[:2]) and (dst[2:] == 3).all()
     with pytest.raises(RuntimeError, match="starts that go back"):
         s.batch.check()
+
+
+def test_check_waits_for_every_stream():
+    """A fault met on another stream than the current one, behind work that takes a while."""
+    s = Setup([(1, 100), (1, 100)], 4, 2, 64, 16, F32, seed=6)
+    a = torch.randn(4096, 4096, device="cuda")
+    side = torch.cuda.Stream()
+    s.cache.attention(s.batch, s.q, stream=side)   # everything is loaded
+    a = a @ a * 1e-3
+    s.batch.check()
+    s.batch.page_table[0, 2] = 12345
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(40):
+            a = a @ a * 1e-3
+    s.cache.attention(s.batch, s.q, stream=side)
+    with pytest.raises(RuntimeError, match="page id"):
+        s.batch.check()
+    s.batch.check()

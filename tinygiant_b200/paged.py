@@ -96,11 +96,14 @@ class PagedBatch:
         self.ref = ctypes.byref(self.c)
 
     def check(self):
-        """Synchronise; raise if a call on this batch since the last check met contents that do
-        not fit the cache (those tokens or rows were left out), and forget it."""
+        """Synchronise the device; raise if a call on this batch since the last check, on whichever
+        stream, met contents that do not fit the cache (those tokens or rows were left out), and
+        forget it."""
+        torch.cuda.synchronize(self.device)   # the calls' streams, whichever they were
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
+            torch.cuda.synchronize(self.device)
             said = [text for bit, text in ((TGX_KVQ_BAD_PAGE, "a page id outside the cache"),
                                            (TGX_KVQ_BAD_LENGTH, "a length beyond the page table or fewer rows than new tokens"),
                                            (TGX_KVQ_BAD_POSITION, "a position outside the rope tables"),
