@@ -365,3 +365,27 @@ def test_device_without_an_index():
     b = BatchedAttention(64, 2, 1, 64, 1, 4, device=0)
     b.fill_synthetic(1)
     assert torch.equal(a.layer(0, batch_of([(2, 2)], width=4), X.clone()), b.layer(0, batch_of([(2, 2)], width=4), X.clone()))
+
+
+def test_experts_that_do_not_go_with_the_layers():
+    """Another width, number of layers or device is refused before anything runs, as are rows that
+    the MoE block cannot take."""
+    from types import SimpleNamespace
+    from tinygiant_b200.serving import BatchedAttention, BatchedEngine
+    a = BatchedAttention(64, 2, 1, 64, 1, 8, 16, 64)
+    a.fill_synthetic(1)
+    X = torch.randn(3, 64, generator=gen(2), device="cuda")
+    before, fits = X.clone(), dict(embed=64, n_layers=1, device=0, top_k=2)
+    a.check_moe(SimpleNamespace(**fits))
+    for bad in (dict(embed=128), dict(n_layers=0), dict(device=1), dict(n_layers=2)):
+        moe = SimpleNamespace(**{**fits, **bad})
+        if moe.n_layers < 2:
+            with pytest.raises(ValueError, match="moe"):
+                a.forward(batch_of([(3, 3)], width=4), X, moe)
+        with pytest.raises(ValueError, match="moe"):
+            BatchedEngine.synthetic(moe, a, 50, 2)
+    wide = torch.randn(3, 128, generator=gen(2), device="cuda")
+    kept = wide.clone()
+    with pytest.raises(ValueError, match="contiguous"):
+        a.forward(batch_of([(3, 3)], width=4), wide[:, :64], SimpleNamespace(**fits))
+    assert torch.equal(X, before) and torch.equal(wide, kept)

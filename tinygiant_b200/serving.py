@@ -18,7 +18,8 @@ from .paged import DTYPES, PagedBatch, PagedKV4, on_stream, stream_handle
 
 class BatchedAttention:
     """X += attention(RMSNorm(X) * attn_norm) for token rows X (cuda float32 [T][embed]); rows
-    behind the batch's last token stay as they are.
+    behind the batch's last token stay as they are (an MoE block knows no batch: forward's takes
+    every row).
 
     One page table serves every layer: page p of a sequence is page p of each layer's cache.
     dtype is the type between the two projections of a layer: float32, or bfloat16 / float16,
@@ -93,11 +94,21 @@ class BatchedAttention:
             return wo(o, out=X, residual=X)
         return X.add_(wo(o))
 
+    def check_moe(self, moe: MoEModel):
+        """Raise unless moe's blocks go with these layers."""
+        if moe.embed != self.embed or moe.n_layers < self.n_layers or moe.device != self.device.index:
+            raise ValueError(f"moe: expected {self.n_layers} layers of width {self.embed} on device {self.device.index}, got "
+                             f"{moe.n_layers} of {moe.embed} on device {moe.device}")
+
     def forward(self, batch: PagedBatch, X, moe: MoEModel | None = None, stream=None):
-        """Every layer on X in place: attention, then moe's MoE block when given."""
+        """Every layer on X in place: attention, then moe's MoE block when given (X contiguous)."""
         if stream is not None:
             with on_stream(stream, self.device):
                 return self.forward(batch, X, moe)
+        if moe is not None:
+            self.check_moe(moe)
+            if not X.is_contiguous():
+                raise ValueError("X: expected contiguous rows in front of an MoE block")
         for l in range(self.n_layers):
             self.layer(l, batch, X)
             if moe is not None:
@@ -112,8 +123,10 @@ class BatchedEngine:
     the final RMSNorm and the output projection of each sequence's last new token."""
 
     def __init__(self, moe: MoEModel | None, attn: BatchedAttention, token_embd, output_norm, output_weight):
-        if moe is not None and (moe.embed != attn.embed or moe.n_layers != attn.n_layers):
-            raise ValueError("moe and attn differ in width or layers")
+        if moe is not None:
+            attn.check_moe(moe)
+            if moe.n_layers != attn.n_layers:
+                raise ValueError("moe and attn differ in layers")
         if token_embd.dtype != torch.float32 or token_embd.dim() != 2 or token_embd.shape[1] != attn.embed:
             raise ValueError(f"token_embd: expected float32 [vocab][{attn.embed}]")
         self.moe, self.attn, self.embd = moe, attn, token_embd.to(attn.device)
