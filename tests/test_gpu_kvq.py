@@ -572,3 +572,16 @@ def test_check_waits_for_every_stream():
     with pytest.raises(RuntimeError, match="page id"):
         s.batch.check()
     s.batch.check()
+
+
+@pytest.mark.parametrize("hd", [64, 96])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_append_leaves_q_alone_without_norm_or_rotation(hd, dtype):
+    """Neither norm nor rope: q comes back as it is, its infinities and NaN in their places."""
+    s = Setup([(3, 9), (2, 20)], 4, 2, hd, 16, dtype, seed=13)
+    q, k, v = append_case(s)[:3]
+    q = q.clone()
+    q[0, 5], q[1, hd // 2 + 1], q[4, 3 * hd + 2] = float("inf"), float("nan"), -float("inf")
+    got = s.cache.append(s.batch, q, k, v).flatten(1)
+    assert torch.equal(torch.isnan(got), torch.isnan(q))
+    assert torch.equal(torch.nan_to_num(got, 7.0), torch.nan_to_num(q, 7.0))

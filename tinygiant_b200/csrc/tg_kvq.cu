@@ -411,6 +411,7 @@ __global__ void __launch_bounds__(32 * WARPS, NB <= 4 ? 3 : NB <= 7 ? 2 : 1) k_k
     if (p < qp) tab.load(cs, sn, a.q_norm, l);
     T* out = reinterpret_cast<T*>(a.q_out) + ((size_t)t * a.NH + 2 * p + side) * HD;
     double* buf = s_buf + (16 % NB ? wid * 32 * N : 0);
+    const bool turns = ok && (a.cos || a.q_norm);   // q is rotated or normalised
     int slot = 0;
 #pragma unroll 1
     for (; p < pairs; p += step, slot = slot + 1 == HELD ? 0 : slot + 1) {
@@ -433,7 +434,10 @@ __global__ void __launch_bounds__(32 * WARPS, NB <= 4 ? 3 : NB <= 7 ? 2 : 1) k_k
                 r = rsqrtf(fmaf(ss, 1.0f / HD, a.eps));
             }
             tab.apply(x, y, r);
-            if (!ok) {
+            if (!turns && ok) {   // as they are: a value must not have met its partner's infinity or NaN times 0
+                load_row(x, row + Q::lower(l));
+                load_row(y, row + Q::upper(l));
+            } else if (!turns) {
 #pragma unroll
                 for (int i = 0; i < NB; i++) x[i] = y[i] = 0.0f;
             }
