@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 
 from tests import serve_ref as R
-from tests.test_gpu_kvq import BF16, F16, Setup, close
+from tests.test_gpu_kvq import BF16, F16, F32, Setup, close
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -239,3 +239,38 @@ def test_queries_that_are_not_finite(dtype):
     assert torch.isnan(got[(hit & ~none).cuda()]).all()
     rest = ~(hit | none).cuda()
     close(got[rest], *[x[rest] for x in s.expect()], 128, 300, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("seqs,nh,nkv,hd", [([(1, 700), (3, 50), (1, 2900)], 8, 2, 128), ([(40, 300), (7, 40)], 16, 2, 64),
+                                            ([(200, 300), (150, 700)] * 4, 16, 2, 128)])
+def test_scores_beyond_the_exponent(seqs, nh, nkv, hd, dtype):
+    """Queries so large that a softmax is one key's: scores of 1e4 to 1e13, where neighbouring fp32
+    numbers are up to 2^20 apart.  The value of the largest score comes out."""
+    s = Setup(seqs, nh, nkv, hd, 64, dtype, seed=21)
+    g = torch.Generator().manual_seed(3)
+    low, high = (3.0, 4.0) if dtype == F16 else (4.0, 12.0)
+    size = 10.0 ** (low + (high - low) * torch.rand(s.T, 1, 1, generator=g)).cuda()
+    s.q = (s.q.double() * size).clamp(-6e4 if dtype == F16 else -1e14, 6e4 if dtype == F16 else 1e14).to(dtype)
+    out = s.cache.attention(s.batch, s.q).double()
+    assert torch.isfinite(out).all()
+    seen = 0
+    for b, (n, r) in enumerate(s.seqs):
+        q, k, v = s.q[s.start[b]:s.start[b + 1]].double(), s.rows(b, s.hk), s.rows(b, s.hv)
+        sees = torch.arange(r, device="cuda")[None] <= (r - n + torch.arange(n, device="cuda"))[:, None]
+        for h in range(nh):
+            j = h // (nh // nkv)
+            score = (q[:, h] @ k[:, j].T * hd ** -0.5).masked_fill(~sees, -float("inf"))
+            size = (q[:, h].abs() @ k[:, j].abs().T * hd ** -0.5).amax(1)
+            best = torch.topk(score, 2, 1)
+            # 11 bits of q and of k, each off by 2^-12 of a product: what lies further apart than both scores'
+            # errors, and 60 besides, decides alone
+            clear = best.values[:, 0] - best.values[:, 1] > 2 * 2 * 2.0 ** -12 * size + 60
+            want = v[best.indices[:, 0], j][clear]
+            got = out[s.start[b]:s.start[b + 1], h][clear]
+            # 11 bits each of p (which is a power of two at the reference only) and of v or p * d, 2^-11 at
+            # most; the roundings of 1 / l and of the products; the type's
+            tol = (2 * 2.0 ** -11 if dtype != F32 else 0) + 2.0 ** -20 + 1.001 * R.EPS[dtype]
+            assert ((got - want).abs() <= tol * want.abs() + 2.0 ** -22).all(), (b, h)
+            seen += int(clear.sum())
+    assert seen > s.T * nh // 4

@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
                 }
             }
             if (lane == 0) {
-                s_fac[r] = a.scale * (RAW ? 0x1p24f : 1.0f) * __uint_as_float((uint32_t)(127 + half) << 23) *
-                           __uint_as_float((uint32_t)(127 + e - half) << 23);
+                s_fac[r] = bounded_fac(a.scale * (RAW ? 0x1p24f : 1.0f) * __uint_as_float((uint32_t)(127 + half) << 23) *
+                                       __uint_as_float((uint32_t)(127 + e - half) << 23));
                 s_lim[r] = ok ? limit(rho / a.R) : 0x7fffffff;   // rows beyond the item: any scores will do
             }
         }
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
             }
         }
 
-        float m[NT][2], off[NT][2], l[NT][2], o[NT][2 * NB][4];   // off = P_EXP - m
+        float m[NT][2], off[NT][2], l[NT][2], o[NT][2 * NB][4];   // m in raw scores; off = P_EXP - m * fac
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
                 }
             }
 
-            // ---- t = s - m + P_EXP; is one beyond the slack in m's range?
+            // ---- t = (s - m) * fac + P_EXP; is one beyond the slack in m's range?
             float t[U][NT][4];
             constexpr uint32_t ALL = (1u << U) - 1;
             const bool edge = t0 + 16 * U > lim_min || (have & ALL) != ALL;
@@ -525,6 +525,7 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
                     vmul = __float2half2_rn(scalbnf(1.0f, -e));
                     vlim = V_HIGH + e >= 16 ? 0x7bffu : (uint32_t)__half_as_ushort(__float2half_rn(scalbnf(1.0f, V_HIGH + e)));
                 }
+                bool beyond = false;
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -534,12 +535,14 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
                         for (int u = 0; u < U; u++)
 #pragma unroll
                             for (int h = 0; h < 2; h++)
-                                if (sees(u, n, k2 + 2 * h)) mn = fmaxf(mn, sc[u][n][k2 + 2 * h] * fac[n][k2]);
+                                if (sees(u, n, k2 + 2 * h)) mn = fmaxf(mn, sc[u][n][k2 + 2 * h]);
 #pragma unroll
                         for (int x = 16; x >= 4; x >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, x));
-                        const float f = mn == m[n][k2] ? 1.0f : ex2(m[n][k2] - mn);
+                        const float f = mn == m[n][k2] ? 1.0f : ex2((m[n][k2] - mn) * fac[n][k2]);
                         m[n][k2] = mn;
-                        off[n][k2] = P_EXP - mn;
+                        const bool far = mn != -INFINITY && fabsf(mn * fac[n][k2]) > FAR;
+                        off[n][k2] = far ? INFINITY : P_EXP - mn * fac[n][k2];   // far: every step comes here
+                        beyond |= far;
                         l[n][k2] *= f;
                         const float of = f * vf;
 #pragma unroll
@@ -550,6 +553,15 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
                     }
                 }
                 place();
+                if (__any_sync(0xffffffffu, beyond)) {
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int x = 0; x < 4; x++)
+                                if (sees(u, n, x)) t[u][n][x] = fmaf(sc[u][n][x] - m[n][x & 1], fac[n][x & 1], P_EXP);
+                }
             }
 
 #pragma unroll
@@ -651,7 +663,7 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
                         row[32 * i + 16 * t + 8 + g] = o[n][2 * i + t][k + 2] * back;
                     }
                 if (g == 0) {
-                    row[HD] = m[n][k];
+                    row[HD] = m[n][k] * fac[n][k];
                     row[HD + 1] = lt * 0x1p-6f;
                 }
             }

@@ -49,6 +49,13 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t x, uint32_t k1024) {
     return as_u32(__hfma2(as_h2(y), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f)));
 }
 
+// 2^score is taken as fma(raw score, fac, offset - fac * reference) while the reference is small, and
+// from the difference of the raw scores where it is so large that fp32 would round the exponent away.
+constexpr float FAR = 65536.0f;
+// A row's factor from raw scores to exponents, kept where products with it are neither 0 nor infinite for
+// sums of at most 2^33: beyond these bounds scores are all alike, or one is all there is.
+__device__ __forceinline__ float bounded_fac(float x) { return fminf(fmaxf(x, 0x1p-120f), 0x1p120f); }
+
 constexpr uint32_t NO_GRANULE = 0xffffffffu;
 
 // N words, in the widest loads that their alignment allows.

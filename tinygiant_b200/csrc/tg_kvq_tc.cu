@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
                 }
             }
             const int e = q_exp(top), half = e / 2;
-            fac = a.scale * pow2(half) * pow2(e - half) * pow2(ex.x);
+            fac = bounded_fac(a.scale * pow2(half) * pow2(e - half) * pow2(ex.x));
             // an infinity's scores may all be -inf, which below is a row without a token to attend to
             l = top >> 23 == 255 && lim > 0 ? __int_as_float(0x7fc00000) : 0.0f;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -319,7 +319,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
         }
         const uint32_t s_at = tmem + q * 128 + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t o_at = tmem + 256 + q * 128 + ((uint32_t)((warp & 3) * 32) << 16);
-        float m = -INFINITY, off = 0.0f;
+        // in raw scores: the reference m, and from where on they leave its range
+        float m = -INFINITY, above = -INFINITY, off = 0.0f;
         bool good = true;
         for (int i = 0; i < tiles && good; i++) {
             good = __all_sync(0xffffffffu, mbar_wait(s_full(q, i), i >> 1 & 1, failed));
@@ -341,11 +342,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
             float top = -INFINITY;
 #pragma unroll
             for (int x = 0; x < TK; x++) top = fmaxf(top, __uint_as_float(v[x / 32][x % 32]));
-            top = top == -INFINITY ? top : top * fac;
-            if (__any_sync(0xffffffffu, top > m + SLACK)) {
-                const float mn = fmaxf(m, top), f = mn == m ? 1.0f : ex2(m - mn);
+            if (__any_sync(0xffffffffu, top > above)) {
+                const float mn = fmaxf(m, top), f = mn == m ? 1.0f : ex2((m - mn) * fac);
                 m = mn;
-                off = m == -INFINITY ? 0.0f : P_EXP - m;
+                const bool far = __any_sync(0xffffffffu, m != -INFINITY && fabsf(m * fac) > FAR);
+                above = far ? -INFINITY : m + __fdividef(SLACK, fac);   // far: every tile comes here
+                off = m == -INFINITY ? 0.0f : far ? P_EXP : P_EXP - m * fac;
                 l *= f;
                 if (i) {
                     good = __all_sync(0xffffffffu, mbar_wait(pv_done(q, i - 1), (i - 1) >> 1 & 1, failed));   // O is at rest
@@ -360,6 +362,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_kvq_tc(TcArgs t) {
                         for (int x = 0; x < 32; x++) w[x] = __float_as_uint(__uint_as_float(w[x]) * f);
                         tmem_st(o_at + c, w);
                     }
+                }
+                if (far) {
+                    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                    for (int x = 0; x < TK; x++) v[x / 32][x % 32] = __float_as_uint(__uint_as_float(v[x / 32][x % 32]) - base);
                 }
             }
             uint32_t p[32];
