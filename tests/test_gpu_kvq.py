@@ -585,3 +585,12 @@ def test_append_leaves_q_alone_without_norm_or_rotation(hd, dtype):
     got = s.cache.append(s.batch, q, k, v).flatten(1)
     assert torch.equal(torch.isnan(got), torch.isnan(q))
     assert torch.equal(torch.nan_to_num(got, 7.0), torch.nan_to_num(q, 7.0))
+
+
+def test_streams_of_another_device_are_refused():
+    from tinygiant_b200.paged import on_stream
+    side = torch.cuda.Stream(device=0)
+    with on_stream(side, torch.device("cuda", 0)), on_stream(side.cuda_stream, torch.device("cuda", 0)):
+        assert torch.cuda.current_stream(0).cuda_stream == side.cuda_stream
+    with pytest.raises(ValueError, match="stream"):
+        on_stream(side, torch.device("cuda", 1))

@@ -44,6 +44,8 @@ def on_stream(stream, device):
     there, and what is allocated belongs to it."""
     if not isinstance(stream, torch.cuda.Stream):
         stream = torch.cuda.ExternalStream(stream, device=device)
+    if stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the call on {device}")
     return torch.cuda.stream(stream)
 
 
