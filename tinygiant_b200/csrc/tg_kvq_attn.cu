@@ -445,18 +445,6 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
             float t[U][NT][4];
             constexpr uint32_t ALL = (1u << U) - 1;
             const bool edge = t0 + 16 * U > lim_min || (have & ALL) != ALL;
-            if (edge) {
-                // V scales that no row of the item sees (an earlier use of the page may have left them) become
-                // 0: they must neither choose vexp nor, beyond fp16 in its units, meet a probability of 0
-                const int left = s_lim[nrows - 1] - t0;
-#pragma unroll 1
-                for (int x = lane; x < U * 8 * NB; x += 32) {   // a word holds two tokens'
-                    const int u = x / (8 * NB), at = x - u * 8 * NB, seen = left - (16 * u + at / NB * 2);
-                    uint32_t* v = reinterpret_cast<uint32_t*>(ring + (k % ST) * (U * GB) + u * GB + 17 * HD) + at;
-                    if (seen < 2) *v = seen == 1 ? *v & 0xffffu : 0u;
-                }
-                __syncwarp();
-            }
             auto sees = [&](int u, int n, int x) {   // whether the column's row attends to the lane's token
                 return t0 + 16 * u + g + 8 * (x >> 1) < lim[n][x & 1] && (have >> (U - 1 - u) & 1);
             };
@@ -500,7 +488,10 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
                 }
             bool mend = false;
             if (__any_sync(0xffffffffu, odd)) {
-                bool nan = false;
+                // What no row of the item sees (an earlier use of the page may have left it) must not choose vexp;
+                // nor, beyond fp16 in its units, meet a probability of 0.
+                const int left = s_lim[nrows - 1] - t0;
+                bool nan = left < 16 * U;
                 float top = 0.0f;   // the largest finite one
 #pragma unroll
                 for (int u = 0; u < U; u++)
@@ -508,7 +499,10 @@ __global__ void __launch_bounds__(32 * DEEP_WARPS, min_ctas(NB, NT)) k_kvq_attn(
                     for (int i = 0; i < (NB + 3) / 4; i++) {
                         const int x = 32 * i + lane;
                         if (x < 8 * NB) {
-                            const __half2 v = __habs2(*reinterpret_cast<const __half2*>(step + u * GB + 17 * HD + 4 * x));
+                            uint32_t w = *reinterpret_cast<const uint32_t*>(step + u * GB + 17 * HD + 4 * x);
+                            const int seen = left - (16 * u + x / NB * 2);   // of the word's two tokens
+                            w = seen >= 2 ? w : seen == 1 ? w & 0xffffu : 0u;
+                            const __half2 v = __habs2(as_h2(w));
                             const float v0 = __low2float(v), v1 = __high2float(v);
                             nan |= !(v0 <= 65504.0f) || !(v1 <= 65504.0f);
                             top = fmaxf(top, fmaxf(v0 <= 65504.0f ? v0 : 0.0f, v1 <= 65504.0f ? v1 : 0.0f));
