@@ -629,7 +629,10 @@ int tgx_kvq_read(const tgx_kvq_cache *cache, const tgx_kvq_batch *batch, int n_t
  * [n_tokens][n_heads * head_dim] of `dtype`, rows *_stride elements apart (4-element aligned;
  * strides multiples of 4); out may be q.  scale: 0 selects 1 / sqrt(head_dim).  A token without a row
  * to attend to (kv_lens 0) gets 0.  n_heads / n_kv_heads <= 32.  Sums and softmax statistics
- * are fp32.  scratch: tgx_kvq_attention_scratch_bytes bytes, 256-byte aligned, no contents
+ * are fp32.  fp32 q: q and probability * scale are held in 22 bits.  16-bit q: probabilities and
+ * code * scale or probability * scale in 11 bits (2^-11 each at most), which float16 outputs show and
+ * bfloat16's own rounding covers; scores good to 2^-11 of sum |q| |k|.  Values are held next to the
+ * largest scale of the rows at hand: blocks more than 2^16 below it lose bits.  scratch: tgx_kvq_attention_scratch_bytes bytes, 256-byte aligned, no contents
  * assumed or kept; calls sharing it must be ordered. */
 size_t tgx_kvq_attention_scratch_bytes(const tgx_kvq_cache *cache, const tgx_kvq_batch *batch, int n_tokens,
                                        int n_heads);

@@ -120,8 +120,8 @@ __device__ __forceinline__ void i8_codes(uint32_t (&c)[V / 4], const float (&x)[
 // over it beat rows held in registers, whose unrolled code did not fit the instruction cache
 // (8100 x 2048 bf16 behind a norm: 41 to 56 us).
 //
-// Bound by the instructions, about 20 an element, for many rows (8100 x 2048: 23 us): a warp each and no barrier
-// (G = 1).  For few rows, by latency: a CTA each (G = 8).
+// Bound by the instructions, 26 issue slots an element, for many rows (8100 x 2048 bf16 behind a norm: 21 us): a
+// warp each and no barrier (G = 1).  For few rows, by latency: a CTA each (G = 8).
 template <int DT, bool NORM, bool VEC, int G>
 __global__ void __launch_bounds__(256, 4) k_i8_rows(QuantArgs a) {
     using T = typename Row<DT>::T;

@@ -10,12 +10,13 @@
 // definition's in 64 bits: computed in 32 with a bound on the error, and where a code, the
 // largest value or the rounding of a scale is within that bound of turning out otherwise (about
 // one pair of heads in 20), once more in 64.  All in 64 bits took 141 us for 13077 tokens of 32
-// and 4 heads of 128.  q has no borders: fp32, rounded once to its type.
+// and 4 heads of 128 in bf16, which now take 90.  q has no borders: fp32, rounded once to its type.
 //
 // 16 lanes per head, 2 NB = HD / 16 dimensions in a row per lane, so the other half of a
 // rotated pair is 8 lanes away, and a block of 32 is 16 / NB lanes.  A warp takes pairs of heads
-// of one kind of one token: angles and norm weights are loaded once for them.  Bound by memory
-// for many tokens: q in and out, k and v in, codes out; by latency for few.
+// of one kind of one token: angles and norm weights are loaded once for them.  Bound by instructions
+// for many tokens: those 13077 take 69 M warp instructions, 33 issue slots an element of q, k and v,
+// where their bytes would take 39 us.  By latency for few.
 #include <algorithm>
 
 #include "tg_serve.cuh"
@@ -465,7 +466,8 @@ __global__ void __launch_bounds__(32 * WARPS, NB <= 4 ? 3 : NB <= 7 ? 2 : 1) k_k
 }
 
 // A warp takes every per_token'th (key or value, kv head) of a token; lane l holds dimensions
-// 32b + l.
+// 32b + l.  A nibble and an element a lane and load: bound by its instructions (13077 tokens of 4
+// heads of 128: 20 us, 3.0 TB/s of codes in and fp32 out).
 template <int NB>
 __global__ void __launch_bounds__(32 * WARPS) k_kvq_read(KvqCache c, KvqBatch bt, int T, int per_token, float* k_out, float* v_out) {
     constexpr int HD = 32 * NB;

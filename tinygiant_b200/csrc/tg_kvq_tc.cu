@@ -24,9 +24,11 @@
 // score MMAs, measured 157 to 183 us again: without a second S a query tile's softmax and MMAs
 // take turns.
 //
-// m moves, and O in TMEM is rescaled, only when a row's scores leave 2^SLACK of it.  q rows, K
-// and V are held in fp16 times powers of two: q's largest in 2^13 .. 2^14, the largest scale of
-// the sequence's head in 2^7 .. 2^8 (found by k_kvq_scan in front, which also marks sequences
+// m moves, and O in TMEM is rescaled, only when a row's scores leave 2^SLACK of it.  m, l and O are
+// fp32.  q rows, K, V and P are held in fp16, the tensor cores' type, 11 bits like the 16-bit inputs (and
+// more than bf16's), times powers of two: q's largest in 2^13 .. 2^14, the largest scale of the
+// sequence's head in 2^7 .. 2^8, so blocks more than 2^21 below it have fewer bits
+// (found by k_kvq_scan in front, which also marks sequences
 // with a scale that is not finite: a NaN behind a row's limit must not meet a probability of 0,
 // so those are left to tg_kvq_attn.cu's kernel).
 //
