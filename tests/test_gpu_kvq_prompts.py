@@ -274,3 +274,18 @@ def test_scores_beyond_the_exponent(seqs, nh, nkv, hd, dtype):
             assert ((got - want).abs() <= tol * want.abs() + 2.0 ** -22).all(), (b, h)
             seen += int(clear.sum())
     assert seen > s.T * nh // 4
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_large_values_behind_the_last_row(dtype):
+    """Finite values with the largest scales in rows that a sequence does not hold change no bit."""
+    s = Setup([(200, 300), (200, 264), (150, 249)] * 3, 16, 2, 128, 64, dtype, seed=2, values=0.05)
+    want = s.cache.attention(s.batch, s.q)
+    used = torch.zeros(s.pages.shape[0], s.page, dtype=torch.bool)
+    for b, (_, r) in enumerate(s.seqs):
+        for i, p in enumerate(s.ids[b]):
+            used[p, :max(0, min(s.page, r - i * s.page))] = True
+    k, v = s.k.clone(), s.v.clone()
+    k[~used.cuda()], v[~used.cuda()] = 5e5, -5e5
+    s.pages.copy_(R.Cache(1, s.nkv, s.hd, s.page).pages(k, v))
+    assert torch.equal(s.cache.attention(s.batch, s.q), want)
